@@ -274,6 +274,134 @@ int qq_set_mfma_min_tokens(qq_ctx *ctx, int tokens);
 int qq_rmsnorm_dev(qq_ctx *ctx, const float *x_dev, const float *weight_dev, float *out_dev, int T,
                    int H, double eps);
 
+/* ---- Paged key/value cache -------------------------------------------------
+ * No counterpart in the reference, whose KVCache (src/kv-cache.js) holds one
+ * sequence: the cache of a program that serves many sequences at once.  A
+ * pool is n_layers x n_pages pages of page_size positions; a sequence is a
+ * row of page numbers (its table) and a length, both in device memory, so a
+ * captured graph follows them as they change between replays.  Pages may be
+ * shared between sequences.
+ *
+ * Layout of the pool: [n_layers][n_pages][2: K, V][n_kv_heads][page_size *
+ * head_dim] values of `type`, in units of 16 bytes (U = 4 values of F32, 8 of
+ * F16 or BF16):
+ *   K  slot s, dimension d at ((d / U) * page_size + s) * U + d % U
+ *   V  slot s, dimension d at ((s / U) * head_dim + d) * U + s % U
+ * A unit of K is U dimensions of one position and a unit of V is U positions
+ * of one dimension: the operands of the matrix instructions that read them.
+ *
+ * page_size 16, 32, 64, 128 or 256; head_dim 32, 64, 96 or 128; type
+ * QQ_TYPE_F32, QQ_TYPE_F16 or QQ_TYPE_BF16. */
+#define QQ_TYPE_F16      1
+#define QQ_TYPE_BF16    30
+typedef struct qq_kv qq_kv;
+
+/* Bytes of such a pool. */
+int qq_kv_pool_bytes(int n_layers, int n_pages, int page_size, int n_kv_heads, int head_dim, int type,
+                     size_t *nbytes);
+/* A pool over the caller's device memory (pool_dev, 16-byte aligned, nbytes
+ * at least qq_kv_pool_bytes; it must outlive the handle, its values are kept)
+ * or, with pool_dev NULL, over zeroed memory of its own.  The handle also
+ * holds the attention's workspace, of a size that no call changes.  Its calls
+ * are made on the context that created it, in the order of that context's
+ * stream. */
+int qq_kv_create(qq_ctx *ctx, void *pool_dev, size_t nbytes, int n_layers, int n_pages, int page_size,
+                 int n_kv_heads, int head_dim, int type, qq_kv **out);
+int qq_kv_release(qq_ctx *ctx, qq_kv *kv);
+/* The pool's device address and size. */
+int qq_kv_pool(const qq_kv *kv, void **pool_dev, size_t *nbytes);
+
+/* The sequences of one call and their new rows.  Rows row_start[b] ..
+ * row_start[b+1] - 1 (row_start not decreasing; NULL: row b alone) are the
+ * last positions of sequence b, whose length len[b] counts them: row i of n
+ * stands at position len[b] - n + i.  Position p lies in slot p % page_size
+ * of page table[b * table_stride + p / page_size].
+ * A row whose position is negative (an idle slot: length 0) is padding.
+ * Positions at or past table_stride * page_size, and those whose table entry
+ * is no page of the pool, are neither written nor seen.  Rows of no sequence
+ * are left as they are. */
+#define QQ_KV_MAX_SEQS 4096
+typedef struct qq_kv_batch {
+    int n_seqs;                    /* at most QQ_KV_MAX_SEQS                  */
+    int n_rows;                    /* rows of q, k, v and out                 */
+    const int32_t *table_dev;      /* [n_seqs][table_stride] page numbers     */
+    int table_stride;              /* table_stride * page_size <= 2^30        */
+    const int32_t *len_dev;        /* [n_seqs]                                */
+    const int32_t *row_start_dev;  /* [n_seqs + 1], or NULL                   */
+} qq_kv_batch;
+
+/* The new rows of an attention block on their way into the cache: per-head
+ * RMSNorm (perHeadRMSNorm, src/tensor.js:117-129) and RoPE (applyRoPE,
+ * :132-147) of q and k, k and v rounded once to the pool's type and written
+ * into layer `layer` at their rows' positions:
+ *   y = fp32(w * x / sqrt(sum x^2 / head_dim + eps))       (norm weight not NULL)
+ *   (y[i], y[i + h]) turned by pos * rope_base^(-i / h), h = head_dim / 2   (rope_base not 0)
+ *   q, q_out [n_rows][n_heads][head_dim]   q_out may be q; both NULL: k and v alone
+ *   k, v     [n_rows][n_kv_heads][head_dim]
+ * binary64 arithmetic.  Padding rows write nothing.  Two rows at one position
+ * of one page leave either's values.  Device pointers; enqueued, not waited for. */
+int qq_kv_store_dev(qq_ctx *ctx, qq_kv *kv, int layer, const qq_kv_batch *batch, const float *q_dev,
+                    int n_heads, const float *k_dev, const float *v_dev, const float *q_norm_dev,
+                    const float *k_norm_dev, double eps, double rope_base, float *q_out_dev);
+
+/* Attention of the batch's rows over their sequences' pages in layer `layer`
+ * (the GQA attention of src/lfm2-engine.js:354-388; query head h reads
+ * key/value head h * n_kv_heads / n_heads, n_heads a multiple of n_kv_heads):
+ * a row at position p sees the positions s <= p of its sequence and, with
+ * window > 0, of these only s > p - window and s < sinks (the first tokens,
+ * which stay visible):
+ *   out = sum_s e^(scale q.k_s - m) v_s / sum_s e^(scale q.k_s - m),  m the largest
+ * A row that sees nothing (padding) gives zeros.
+ *   q, out [n_rows][n_heads][head_dim] fp32; out must not overlap q
+ * q enters its products exactly with a BF16 or F32 pool and to 22 bits beside
+ * each head's largest with an F16 one, as the probabilities do; sums are fp32.
+ * A visible key or value that is not finite makes its rows' heads NaN or
+ * infinite; invisible ones have no effect.  Rows may be many (prompt chunks)
+ * or one a sequence (decode); the work is split over the context's length
+ * where rows are few, by the lengths in device memory.  Device pointers;
+ * enqueued, not waited for. */
+int qq_kv_attn_dev(qq_ctx *ctx, qq_kv *kv, int layer, const qq_kv_batch *batch, const float *q_dev,
+                   int n_heads, double scale, int window, int sinks, float *out_dev);
+
+/* pool[pairs[i][1]] = pool[pairs[i][0]], K and V of every layer, for n pairs of
+ * page numbers (int32 [n][2], device memory).  A pair with a number that is
+ * no page of the pool is skipped.  No page may be the destination of two
+ * pairs, or the destination of one and the source of another.  Enqueued. */
+int qq_kv_copy_pages_dev(qq_ctx *ctx, qq_kv *kv, const int32_t *pairs_dev, int n);
+/* table[i] = map[table[i]] for n entries; entries outside [0, n_map) stay.
+ * map must not overlap table.  Device pointers; enqueued, not waited for. */
+int qq_kv_remap_dev(qq_ctx *ctx, int32_t *table_dev, int n, const int32_t *map_dev, int n_map);
+
+/* Which page belongs to whom: book-keeping in host memory, without a device
+ * (failures are reported by qq_last_error(NULL)).  It hands out page numbers
+ * and counts their users; the caller uploads the tables and runs the copies
+ * it is told to.  Not for use by two threads at once. */
+typedef struct qq_pages qq_pages;
+int qq_pages_create(int n_pages, int page_size, qq_pages **out);
+int qq_pages_release(qq_pages *p);
+/* An empty sequence; *seq is its number from then on. */
+int qq_pages_new(qq_pages *p, int *seq);
+/* n more positions for a sequence.  Positions that would fall into a page
+ * with other users get a page of their own: pair[0] -> pair[1] is then to be
+ * copied ahead of the next store (*n_pairs = 1, else 0).  QQ_E_NOMEM, and
+ * nothing changed, when too few pages are free. */
+int qq_pages_extend(qq_pages *p, int seq, int n, int32_t *pair, int *n_pairs);
+/* A new sequence that shares the pages of the first len positions of `seq`. */
+int qq_pages_fork(qq_pages *p, int seq, int len, int *out_seq);
+/* Keep the first len positions; pages behind them lose this user. */
+int qq_pages_truncate(qq_pages *p, int seq, int len);
+int qq_pages_free(qq_pages *p, int seq);
+/* The sequence's length, its page count, and its table row: `cap` entries, -1
+ * behind its pages (row NULL: the counts alone). */
+int qq_pages_table(const qq_pages *p, int seq, int32_t *row, int cap, int *n, int *len);
+/* Move the used pages to the lowest numbers: pairs (int32 [cap][2]) for
+ * qq_kv_copy_pages_dev, and in map (n_pages entries, or NULL) every page's new
+ * number for qq_kv_remap_dev.  The sequences' rows have the new numbers from
+ * then on.  QQ_E_ARG, and nothing changed, when cap is too small: it never is
+ * at the smaller of the free and the used count. */
+int qq_pages_compact(qq_pages *p, int32_t *pairs, int cap, int *n_pairs, int32_t *map);
+int qq_pages_count(const qq_pages *p, int *n_free, int *n_used);
+
 /* ---- measurement ------------------------------------------------------ */
 
 /* Record a HIP event pair around work enqueued between qq_timer_start and

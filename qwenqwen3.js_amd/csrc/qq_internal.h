@@ -114,7 +114,26 @@ struct qq_moe {
     qq_tensor *owned[3];                 // ... unless the layer owns them (GGUF loader)
 };
 
-namespace qq { struct DecodeLayer; }
+namespace qq {
+
+struct DecodeLayer;
+
+// A paged key/value cache's shape (include/qq_moe.h has the layout).
+constexpr int KV_MAX_DIM = 128;
+struct KvShape {
+    int n_layers, n_pages, page_size, page_log, n_kv_heads, head_dim, type;
+    size_t page_bytes;   // K and V of one page of one layer
+};
+
+}  // namespace qq
+
+struct qq_kv {
+    qq_ctx *ctx = nullptr;
+    qq::KvShape s{};
+    char *pool = nullptr;
+    size_t nbytes = 0;
+    bool own_pool = false;
+};
 
 // Layers of one MoE stack (qq_moe_stack_create): borrowed layer handles, their
 // ffn_norm weights, and the decode kernel's device table of their pointers.
@@ -203,6 +222,10 @@ enum KernelId {
     K_LFM2_ATTN,
     K_ROUTE_DISPATCH,
     K_ROW_INV,
+    K_KV_STORE,
+    K_KV_ATTN,
+    K_KV_JOIN,
+    K_KV_PAGES,
     K_COUNT
 };
 
@@ -391,6 +414,31 @@ int launch_moe_stream(qq_ctx *ctx, const qq_moe *m, const float *x, float *hidde
                       bool dispatched = false);
 int launch_rmsnorm(qq_ctx *ctx, const float *x, const float *w, float *out, int T, int H,
                    double eps);
+// One call's batch over one layer of a paged cache, by value to its kernels.
+struct KvBatch {
+    KvShape s;
+    char *pool;   // the layer's pages
+    const int32_t *table, *len, *row_start;
+    int n_seqs, n_rows, stride;
+};
+struct KvStore {
+    const float *q, *k, *v, *qn, *kn;
+    float *q_out;
+    int n_heads;    // 0: no q
+    int rope;
+    double eps;
+    double freq[KV_MAX_DIM / 2];
+};
+struct KvAttn {
+    const float *q;
+    float *out;
+    int n_heads, group, window, sinks;   // window 0: none; group query heads a key/value head
+    double scale;
+};
+int launch_kv_store(qq_ctx *ctx, const KvBatch &b, const KvStore &st);
+int launch_kv_attn(qq_ctx *ctx, const qq_kv *kv, const KvBatch &b, const KvAttn &a);
+int launch_kv_copy(qq_ctx *ctx, const KvShape &s, char *pool, const int32_t *pairs, int n);
+int launch_kv_remap(qq_ctx *ctx, int32_t *table, int n, const int32_t *map, int n_map);
 int launch_moe_grouped(qq_ctx *ctx, const qq_moe *m, const float *x, float *hidden, int T,
                        const MaskBits &mask, const int32_t *idx, const double *w, char *work);
 

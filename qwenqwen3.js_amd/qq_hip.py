@@ -19,7 +19,10 @@ LIB_PATH = os.path.join(_HERE, "libqqmoe.so")
 
 QQ_OK = 0
 TYPE_F32 = 0
+TYPE_F16 = 1
 TYPE_Q8_0 = 8
+TYPE_BF16 = 30
+KV_MAX_SEQS = 4096
 GATING_SIGMOID_BIAS = 0   # LFM2-MoE
 GATING_SOFTMAX = 1        # Qwen3-MoE
 QQ_WAIT_LIMIT_US_DEFAULT = 50000
@@ -38,6 +41,10 @@ EXPORTS = (
     "qq_profile_enable", "qq_profile_read", "qq_profile_name", "qq_profile_kernel_count",
     "qq_capture_begin", "qq_capture_end", "qq_graph_launch", "qq_graph_release",
     "qq_buffer_alloc", "qq_buffer_free", "qq_buffer_write", "qq_buffer_read", "qq_moe_forward_record_dev",
+    "qq_kv_pool_bytes", "qq_kv_create", "qq_kv_release", "qq_kv_pool", "qq_kv_store_dev", "qq_kv_attn_dev",
+    "qq_kv_copy_pages_dev", "qq_kv_remap_dev",
+    "qq_pages_create", "qq_pages_release", "qq_pages_new", "qq_pages_extend", "qq_pages_fork", "qq_pages_truncate",
+    "qq_pages_free", "qq_pages_table", "qq_pages_compact", "qq_pages_count",
 )
 # ... and include/qq_gguf.h
 GGUF_EXPORTS = (
@@ -61,6 +68,15 @@ class Lfm2Info(ctypes.Structure):
         "n_layers", "n_embd", "n_heads", "n_head_kv", "head_dim", "n_vocab", "n_ff", "n_experts",
         "n_experts_used", "n_dense_lead", "l_cache", "max_ctx", "n_attn_layers")] + [
         ("eps", ctypes.c_double), ("rope_freq_base", ctypes.c_double)]
+
+
+class KvBatch(ctypes.Structure):
+    """The sequences of one call on a paged cache and their new rows (qq_kv_batch): device addresses as integers."""
+    _fields_ = [("n_seqs", ctypes.c_int), ("n_rows", ctypes.c_int), ("table_dev", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int), ("len_dev", ctypes.c_void_p), ("row_start_dev", ctypes.c_void_p)]
+
+    def __init__(self, n_seqs, table_ptr, table_stride, len_ptr, row_start_ptr=None, n_rows=None):
+        super().__init__(n_seqs, n_seqs if n_rows is None else n_rows, table_ptr, table_stride, len_ptr, row_start_ptr)
 
 
 class GgufHeader(ctypes.Structure):
@@ -135,6 +151,24 @@ def load():
         "qq_buffer_write": (I, [P, P, P, S]),
         "qq_buffer_read": (I, [P, P, P, S]),
         "qq_moe_forward_record_dev": (I, [P, P, P, P, I, P, P]),
+        "qq_kv_pool_bytes": (I, [I, I, I, I, I, I, ctypes.POINTER(S)]),
+        "qq_kv_create": (I, [P, P, S, I, I, I, I, I, I, PP]),
+        "qq_kv_release": (I, [P, P]),
+        "qq_kv_pool": (I, [P, PP, ctypes.POINTER(S)]),
+        "qq_kv_store_dev": (I, [P, P, I, P, P, I, P, P, P, P, ctypes.c_double, ctypes.c_double, P]),
+        "qq_kv_attn_dev": (I, [P, P, I, P, P, I, ctypes.c_double, I, I, P]),
+        "qq_kv_copy_pages_dev": (I, [P, P, P, I]),
+        "qq_kv_remap_dev": (I, [P, P, I, P, I]),
+        "qq_pages_create": (I, [I, I, PP]),
+        "qq_pages_release": (I, [P]),
+        "qq_pages_new": (I, [P, ctypes.POINTER(I)]),
+        "qq_pages_extend": (I, [P, I, I, P, ctypes.POINTER(I)]),
+        "qq_pages_fork": (I, [P, I, I, ctypes.POINTER(I)]),
+        "qq_pages_truncate": (I, [P, I, I]),
+        "qq_pages_free": (I, [P, I]),
+        "qq_pages_table": (I, [P, I, P, I, ctypes.POINTER(I), ctypes.POINTER(I)]),
+        "qq_pages_compact": (I, [P, P, I, ctypes.POINTER(I), P]),
+        "qq_pages_count": (I, [P, ctypes.POINTER(I), ctypes.POINTER(I)]),
         "qq_gguf_open": (I, [ctypes.c_char_p, PP]),
         "qq_gguf_open_memory": (I, [P, S, PP]),
         "qq_gguf_close": (None, [P]),
@@ -295,6 +329,18 @@ class Context:
         self.check(self.L.qq_profile_read(self.h, _ptr(ms), _ptr(cnt), n), "qq_profile_read")
         return {self.L.qq_profile_name(i).decode(): (float(ms[i]), int(cnt[i]))
                 for i in range(n) if cnt[i]}
+
+    # ---- paged key/value cache ----
+    def kv_pool(self, n_layers, n_pages, page_size, n_kv_heads, head_dim, type=TYPE_F32, ptr=None, nbytes=0):
+        """A paged cache over device memory at `ptr` (nbytes of it), or over zeroed memory of its own (qq_kv_create)."""
+        h = ctypes.c_void_p()
+        self.check(self.L.qq_kv_create(self.h, ptr, nbytes, n_layers, n_pages, page_size, n_kv_heads, head_dim, type,
+                                       ctypes.byref(h)), "qq_kv_create")
+        return KvPool(self, h)
+
+    def kv_remap_dev(self, table_ptr, n, map_ptr, n_map):
+        """table[i] = map[table[i]] for n entries, device pointers (qq_kv_remap_dev)."""
+        self.check(self.L.qq_kv_remap_dev(self.h, table_ptr, n, map_ptr, n_map), "qq_kv_remap_dev")
 
     # ---- tensors ----
     def upload_q8_0(self, gguf_bytes, in_dim, out_dim, n_mats=1):
@@ -471,6 +517,106 @@ class Lfm2Model:
     def release(self):
         if self.h:
             self.L.qq_lfm2_release(self.ctx.h, self.h)
+            self.h = None
+
+
+class KvPool:
+    """The pages of a key/value cache (qq_kv_*); device pointers, enqueued."""
+
+    def __init__(self, ctx, h):
+        self.ctx, self.h = ctx, h
+        ptr, n = ctypes.c_void_p(), ctypes.c_size_t()
+        ctx.check(ctx.L.qq_kv_pool(h, ctypes.byref(ptr), ctypes.byref(n)), "qq_kv_pool")
+        self.ptr, self.nbytes = ptr.value, n.value
+
+    def store_dev(self, layer, batch, k_ptr, v_ptr, q_ptr=None, n_heads=0, q_norm_ptr=None, k_norm_ptr=None, eps=1e-5,
+                  rope_base=0.0, q_out_ptr=None):
+        """The new rows' q and k normed and turned, k and v into their pages (qq_kv_store_dev)."""
+        self.ctx.check(self.ctx.L.qq_kv_store_dev(self.ctx.h, self.h, layer, ctypes.byref(batch), q_ptr, n_heads, k_ptr,
+                                                  v_ptr, q_norm_ptr, k_norm_ptr, eps, rope_base, q_out_ptr),
+                       "qq_kv_store_dev")
+
+    def attn_dev(self, layer, batch, q_ptr, n_heads, out_ptr, scale, window=0, sinks=0):
+        """Attention of the new rows over their sequences' pages (qq_kv_attn_dev)."""
+        self.ctx.check(self.ctx.L.qq_kv_attn_dev(self.ctx.h, self.h, layer, ctypes.byref(batch), q_ptr, n_heads, scale,
+                                                 window, sinks, out_ptr), "qq_kv_attn_dev")
+
+    def copy_pages_dev(self, pairs_ptr, n):
+        """pool[dst] = pool[src] for n (src, dst) pairs (qq_kv_copy_pages_dev)."""
+        self.ctx.check(self.ctx.L.qq_kv_copy_pages_dev(self.ctx.h, self.h, pairs_ptr, n), "qq_kv_copy_pages_dev")
+
+    def release(self):
+        if self.h:
+            self.ctx.check(self.ctx.L.qq_kv_release(self.ctx.h, self.h), "qq_kv_release")
+            self.h = None
+
+
+class Pages:
+    """Which sequence uses which page (qq_pages_*): host memory, no device."""
+
+    def __init__(self, n_pages, page_size):
+        self.L = load()
+        self.h = ctypes.c_void_p()
+        self.n_pages, self.page_size = n_pages, page_size
+        self._check(self.L.qq_pages_create(n_pages, page_size, ctypes.byref(self.h)), "qq_pages_create")
+
+    def _check(self, rc, what):
+        if rc != QQ_OK:
+            raise QQError("%s failed (%d): %s" % (what, rc, self.L.qq_last_error(None).decode()))
+
+    def new(self):
+        seq = ctypes.c_int()
+        self._check(self.L.qq_pages_new(self.h, ctypes.byref(seq)), "qq_pages_new")
+        return seq.value
+
+    def extend(self, seq, n):
+        """n more positions; the (src, dst) pages to copy before the next store, or None."""
+        pair, k = (ctypes.c_int32 * 2)(), ctypes.c_int()
+        self._check(self.L.qq_pages_extend(self.h, seq, n, pair, ctypes.byref(k)), "qq_pages_extend")
+        return (pair[0], pair[1]) if k.value else None
+
+    def fork(self, seq, length):
+        out = ctypes.c_int()
+        self._check(self.L.qq_pages_fork(self.h, seq, length, ctypes.byref(out)), "qq_pages_fork")
+        return out.value
+
+    def truncate(self, seq, length):
+        self._check(self.L.qq_pages_truncate(self.h, seq, length), "qq_pages_truncate")
+
+    def free(self, seq):
+        self._check(self.L.qq_pages_free(self.h, seq), "qq_pages_free")
+
+    def length(self, seq):
+        n = ctypes.c_int()
+        self._check(self.L.qq_pages_table(self.h, seq, None, 0, None, ctypes.byref(n)), "qq_pages_table")
+        return n.value
+
+    def table(self, seq, width=None):
+        """The sequence's page numbers (int32), -1 up to `width`."""
+        n = ctypes.c_int()
+        self._check(self.L.qq_pages_table(self.h, seq, None, 0, ctypes.byref(n), None), "qq_pages_table")
+        row = np.empty(n.value if width is None else width, np.int32)
+        self._check(self.L.qq_pages_table(self.h, seq, _ptr(row), row.size, None, None), "qq_pages_table")
+        return row
+
+    def compact(self):
+        """(pairs int32 [n, 2] to copy, map int32 [n_pages] of the tables' entries)."""
+        free, used = self.count()
+        pairs, k = np.empty((max(1, min(free, used)), 2), np.int32), ctypes.c_int()
+        to = np.empty(self.n_pages, np.int32)
+        self._check(self.L.qq_pages_compact(self.h, _ptr(pairs), pairs.shape[0], ctypes.byref(k), _ptr(to)),
+                    "qq_pages_compact")
+        return pairs[:k.value].copy(), to
+
+    def count(self):
+        """(free, used) pages."""
+        a, b = ctypes.c_int(), ctypes.c_int()
+        self._check(self.L.qq_pages_count(self.h, ctypes.byref(a), ctypes.byref(b)), "qq_pages_count")
+        return a.value, b.value
+
+    def release(self):
+        if self.h:
+            self.L.qq_pages_release(self.h)
             self.h = None
 
 
