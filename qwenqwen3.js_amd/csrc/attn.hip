@@ -1,111 +1,580 @@
-// attn.hip -- attention of new rows over the pages of a key/value cache.
+// attn.hip -- attention of new rows over the pages of a key/value cache:
+// softmax(scale q K^T) V with the running maximum and sum of a softmax, in
+// one pass over the keys and values a row sees.
 //
-// One wave per (row, query head): 64 positions a step, a lane each for the
-// scores, then a lane per dimension for the sum over values, with the running
-// maximum and sum of a softmax (fp32).
+// A key/value head's query heads and rows are the 16 columns of one matrix
+// product: a wave takes a step of 4 U positions (U values in 16 bytes: 16
+// positions of fp32, 32 of the 16-bit types) and forms
+//     S^T [positions x columns] = K Q^T,   O^T [dimensions x columns] += V^T P^T
+// with 16x16 matrix instructions.  Lane l of a wave stands for column l % 16;
+// j = l / 16 picks the unit of the inner index.  The result of the first
+// product leaves lane (column, j) with the scores of 4 positions per
+// instruction, and the second wants, in the same lane, the probabilities of U
+// consecutive positions, unit j of the step.  Which position is which row of
+// K's operand is free, so row m of instruction x is position U (m / 4) + 4 x +
+// m % 4 of the step: the scores then are in the lane that needs them, and
+// nothing moves between lanes but a maximum over j.  The operands come
+// straight from the pool, 16 bytes a lane: its layout is the instructions'.
+//
+// Precision: a product of a 16-bit key with an fp32 query is exact where the
+// query is taken as planes of that type (three of bf16, cut, 24 bits; two of
+// fp16, rounded, 22 bits beside the column's largest, which is scaled to
+// 2^14), and the same goes for probabilities (fp16: scaled by 2^14) and
+// values; sums are fp32.  The matrix pipes are far from the bound here: the
+// cache's bytes are.
+//
+// Work: all steps of the call in a row -- sequences, key/value heads, column
+// tiles, each tile's span -- are cut into equal parts, one a workgroup,
+// wherever the cuts fall (kv_plan.h); lengths are read on the device.  A
+// workgroup's waves take its steps in turn and join in LDS; what a cut
+// separates goes to the workspace, two slots a workgroup (a tile it goes on
+// with from the workgroup before it, and one it leaves to the next), and a
+// second launch joins those.
 #include "kv_device.h"
+#include "kv_plan.h"
 
 namespace qq {
 
-__device__ __forceinline__ float wave_maxf(float v)
+typedef float f4_t __attribute__((ext_vector_type(4)));
+typedef float f4u_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
+
+constexpr int AT_COLS = 16;      // columns of a tile
+constexpr int AT_WAVES = 4;      // waves of a workgroup
+constexpr int AT_THREADS = AT_WAVES * WAVE;
+constexpr int AT_PER_CU = 2;     // workgroups a CU holds
+
+static int attn_parts(const qq_ctx *ctx) { return std::min(ctx->num_cus * AT_PER_CU, 4095); }
+// floats of a workspace slot: 16 columns of D sums, their maxima and sums of probabilities
+__host__ __device__ constexpr int attn_slot(int dim) { return AT_COLS * (dim + 2); }
+size_t kv_attn_work_bytes(const qq_ctx *ctx, const KvShape &s)
 {
+    return (size_t)attn_parts(ctx) * 2 * attn_slot(s.head_dim) * sizeof(float);
+}
+
+// ---- operands by cache type: q's planes, a step's probabilities -------------------
+
+// Fp32 keys and values: 16x16x4 instructions, one per element of the 16 bytes.
+template <class E>
+struct AtOps {
+    static constexpr float PSHIFT = 0.0f;
+    struct Q {
+        float v[4];
+    };
+    typedef Q P;
+    static __device__ __forceinline__ Q split(const float (&x)[4]) { return Q{{x[0], x[1], x[2], x[3]}}; }
+    static __device__ __forceinline__ f4_t mul(const uint4 &a, const Q &q, f4_t c)
+    {
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, WAVE));
-    return v;
+        for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w[i]), q.v[i], c, 0, 0, 0);
+        return c;
+    }
+};
+
+template <>
+struct AtOps<KvBf16> {
+    static constexpr float PSHIFT = 0.0f;
+    struct Q {
+        b8_t h, m, l;   // x = h + m + l
+    };
+    typedef Q P;
+    static __device__ __forceinline__ Q split(const float (&x)[8])
+    {
+        uint32_t h[4], m[4], l[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            uint32_t a = __float_as_uint(x[2 * i]), b = __float_as_uint(x[2 * i + 1]);
+            float ra = x[2 * i] - __uint_as_float(a & 0xffff0000u), rb = x[2 * i + 1] - __uint_as_float(b & 0xffff0000u);
+            h[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);   // the high halves
+            a = __float_as_uint(ra);
+            b = __float_as_uint(rb);
+            ra -= __uint_as_float(a & 0xffff0000u);
+            rb -= __uint_as_float(b & 0xffff0000u);
+            m[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            l[i] = __builtin_amdgcn_perm(__float_as_uint(rb), __float_as_uint(ra), 0x07060302u);
+        }
+        Q q;
+        q.h = __builtin_bit_cast(b8_t, make_uint4(h[0], h[1], h[2], h[3]));
+        q.m = __builtin_bit_cast(b8_t, make_uint4(m[0], m[1], m[2], m[3]));
+        q.l = __builtin_bit_cast(b8_t, make_uint4(l[0], l[1], l[2], l[3]));
+        return q;
+    }
+    static __device__ __forceinline__ f4_t mul(const uint4 &a, const Q &q, f4_t c)
+    {
+        const b8_t v = __builtin_bit_cast(b8_t, a);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, q.l, c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, q.m, c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, q.h, c, 0, 0, 0);
+    }
+};
+
+template <>
+struct AtOps<KvF16> {
+    static constexpr float PSHIFT = 14.0f;   // probabilities up to 2^14: 2^-39 of the largest is still told apart
+    struct Q {
+        h8_t h, l;   // x = h + l to 22 bits
+    };
+    typedef Q P;
+    static __device__ __forceinline__ Q split(const float (&x)[8])
+    {
+        Q q;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            q.h[i] = (_Float16)x[i];
+            q.l[i] = (_Float16)(x[i] - (float)q.h[i]);
+        }
+        return q;
+    }
+    static __device__ __forceinline__ f4_t mul(const uint4 &a, const Q &q, f4_t c)
+    {
+        const h8_t v = __builtin_bit_cast(h8_t, a);
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, q.l, c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(v, q.h, c, 0, 0, 0);
+    }
+};
+
+// ---- lanes ------------------------------------------------------------------------
+
+__device__ __forceinline__ float f_of(uint32_t v) { return __uint_as_float(v); }
+
+// Maximum, or sum, over the four lanes of one column (l, l ^ 16, l ^ 32, l ^ 48).
+__device__ __forceinline__ float col_max(float v)
+{
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(f_of(a[0]), f_of(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(f_of(b[0]), f_of(b[1]));
+}
+__device__ __forceinline__ float col_sum(float v)
+{
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = f_of(a[0]) + f_of(a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f_of(b[0]) + f_of(b[1]);
+}
+
+// ---- the plan, in every workgroup ---------------------------------------------------
+
+struct AtTile {
+    int seq, head, t;        // sequence, key/value head, column tile
+    int row0, rows, len;     // the sequence's new rows and length
+    uint64_t start;          // the tile's first step among the call's
+    KvSpan span;
+};
+
+template <int SLOG>
+__device__ __forceinline__ KvSpan at_span(const KvBatch &b, const KvAttn &a, int len, int rows, int t)
+{
+    return kv_tile_span(len, rows, t, AT_COLS, a.group, b.stride << b.s.page_log, a.window, a.sinks, SLOG);
+}
+
+// pre[i] = steps of the sequences ahead of i, for i <= n_seqs (threads: the whole workgroup).
+template <int SLOG, int NT>
+__device__ __forceinline__ void at_prefix(const KvBatch &b, const KvAttn &a, uint64_t *pre, uint64_t *red)
+{
+    const int per = (b.n_seqs + NT - 1) / NT, tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
+    const int s0 = min(tid * per, b.n_seqs), s1 = min(s0 + per, b.n_seqs);
+    uint64_t sum = 0;
+    for (int s = s0; s < s1; s++) {
+        int r0, r1;
+        kv_rows(b, s, r0, r1);
+        const int len = max(b.len[s], 0), n = kv_tiles(r1 - r0, a.group, AT_COLS);
+        uint64_t steps = 0;
+        for (int t = 0; t < n; t++) steps += at_span<SLOG>(b, a, len, r1 - r0, t).n;
+        pre[s] = sum;      // within this thread's run
+        sum += steps * b.s.n_kv_heads;
+    }
+    uint64_t inc = sum;
+#pragma unroll
+    for (int o = 1; o < WAVE; o <<= 1) {
+        const uint64_t up = __shfl_up(inc, o, WAVE);
+        if (lane >= o) inc += up;
+    }
+    if (lane == WAVE - 1) red[wave] = inc;
+    __syncthreads();
+    uint64_t off = inc - sum;
+    for (int w = 0; w < wave; w++) off += red[w];
+    for (int s = s0; s < s1; s++) pre[s] += off;
+    if (tid == NT - 1) pre[b.n_seqs] = off + sum;
+    __syncthreads();
+}
+
+// The tile that holds step x.
+template <int SLOG>
+__device__ __forceinline__ AtTile at_find(const KvBatch &b, const KvAttn &a, const uint64_t *pre, uint64_t x)
+{
+    int lo = 0, hi = b.n_seqs - 1;   // the last sequence that starts at or ahead of x
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (pre[mid] <= x) lo = mid;
+        else hi = mid - 1;
+    }
+    AtTile t;
+    t.seq = lo;
+    int r1;
+    kv_rows(b, lo, t.row0, r1);
+    t.rows = r1 - t.row0;
+    t.len = max(b.len[lo], 0);
+    const uint64_t per = (pre[lo + 1] - pre[lo]) / b.s.n_kv_heads, r = x - pre[lo];
+    t.head = (int)(r / per);
+    t.start = pre[lo] + per * t.head;
+    for (t.t = 0;; t.t++) {
+        t.span = at_span<SLOG>(b, a, t.len, t.rows, t.t);
+        if (x < t.start + t.span.n) return t;
+        t.start += t.span.n;
+    }
+}
+
+// ---- the kernel ---------------------------------------------------------------------
+
+template <class E, int D>
+__global__ __launch_bounds__(AT_THREADS, AT_PER_CU) void kv_attn_kernel(KvBatch b, KvAttn a, float *__restrict__ work)
+{
+    typedef AtOps<E> Ops;
+    constexpr int U = E::U, TK = U / 4, DS = D / (4 * U), DT = D / 16;
+    constexpr int STEP = 4 * U, SLOG = U == 4 ? 4 : 5;
+    constexpr int LDO = D + 4;   // floats of a column in LDS: the four lanes of a column 16 bytes apart, columns over all banks
+    extern __shared__ uint64_t pre[];
+    __shared__ __align__(16) float so[AT_WAVES][AT_COLS][LDO];
+    __shared__ float sm[AT_WAVES][AT_COLS], sl[AT_WAVES][AT_COLS];
+    __shared__ uint64_t red[AT_WAVES];
+    at_prefix<SLOG, AT_THREADS>(b, a, pre, red);
+    const uint64_t W = pre[b.n_seqs];
+    if (W == 0) return;
+    const uint32_t n = kv_parts(W, gridDim.x, AT_WAVES);
+    if (blockIdx.x >= n) return;
+    const uint64_t x1 = kv_cut(W, n, blockIdx.x + 1);
+    const uint64_t x0 = kv_cut(W, n, blockIdx.x);
+
+    const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
+    const int col = lane & 15, j = lane >> 4;
+    const int nkv = b.s.n_kv_heads, ps = b.s.page_size, nh = a.n_heads, grp = a.group;
+    // K's operand row `col` is a position of unit ku; its unit of dimensions is j + 4 s
+    const int ku = col >> 2, kp = U * ku + (col & 3);
+    const size_t vbase = (size_t)nkv * ps * D * (16 / U);
+    const float qscale = (float)(a.scale * 1.4426950408889634);   // probabilities are powers of two
+
+    for (uint64_t x = x0; x < x1;) {
+        const AtTile t = at_find<SLOG>(b, a, pre, x);
+        const int i0 = (int)(x - t.start);
+        const uint64_t tend = t.start + t.span.n;
+        const int i1 = (int)((tend < x1 ? tend : x1) - t.start);
+        const int c0 = t.t * AT_COLS, ncol = min(AT_COLS, t.rows * grp - c0);
+        // rows of the tile's columns, and their positions
+        const int p0 = t.len - t.rows + c0 / grp, p1 = t.len - t.rows + (c0 + ncol - 1) / grp;
+        const int cr = (c0 + col) / grp;
+        const bool live = col < ncol;
+        const int pos = live ? t.len - t.rows + cr : -1;
+        const int low = a.window && pos >= 0 ? max(pos - a.window + 1, 0) : 0;
+        const int low0 = a.window && p0 >= 0 ? max(p0 - a.window + 1, 0) : 0;   // what the tile's first ...
+        const int low1 = a.window && p1 >= 0 ? max(p1 - a.window + 1, 0) : 0;   // ... and last row's windows start with
+        const int sinks = a.sinks;
+
+        // ---- q in planes ----
+        typename Ops::Q q[DS];
+        float unscale = 1.0f;
+        {
+            float v[DS][U];
+            const float *src = a.q + ((size_t)(t.row0 + cr) * nh + t.head * grp + (c0 + col) % grp) * D;
+            float big = 0.0f;
+#pragma unroll
+            for (int s = 0; s < DS; s++)
+#pragma unroll
+                for (int e = 0; e < U; e++) {
+                    v[s][e] = live ? src[(4 * s + j) * U + e] * qscale : 0.0f;
+                    big = fmaxf(big, fabsf(v[s][e]));
+                }
+            if (Ops::PSHIFT != 0.0f) {
+                // the largest to [2^14, 2^15)
+                const int f = min(268 - (int)(__float_as_uint(col_max(big)) >> 23), 253);
+                unscale = __uint_as_float((uint32_t)(254 - f) << 23);
+                const float up = __uint_as_float((uint32_t)f << 23);
+#pragma unroll
+                for (int s = 0; s < DS; s++)
+#pragma unroll
+                    for (int e = 0; e < U; e++) v[s][e] *= up;
+            }
+#pragma unroll
+            for (int s = 0; s < DS; s++) q[s] = Ops::split(v[s]);
+        }
+
+        float m = -INFINITY, l = 0.0f;
+        f4_t o[DT];
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[d] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+
+        // One step's operands in registers.  Keys are loaded for the next step
+        // once this step's scores are formed, values once its sums are: each
+        // has the other half of a step to arrive in.  (Table entries are read
+        // a step ahead of the loads that need them.)
+        uint4 fk[TK][DS], fv[DT];
+        auto pages = [&](int i, int &gk, int &gv) {
+            const int base = kv_base(t.span, min(i, i1 - 1), SLOG);
+            gk = kv_page(b, t.seq, base + U * ku);
+            gv = kv_page(b, t.seq, base + U * j);
+        };
+        auto load_k = [&](int i, int g) {
+            const int ks = (kv_base(t.span, min(i, i1 - 1), SLOG) + kp) & (ps - 1);
+            const char *src = b.pool + (size_t)max(g, 0) * b.s.page_bytes + ((size_t)(t.head * (D / U) + j) * ps + ks) * 16;
+#pragma unroll
+            for (int s = 0; s < DS; s++)
+#pragma unroll
+                for (int xx = 0; xx < TK; xx++)
+                    fk[xx][s] = *reinterpret_cast<const uint4 *>(src + (size_t)s * 64 * ps + 64 * xx);
+        };
+        auto load_v = [&](int i, int g) {
+            const int vs = (kv_base(t.span, min(i, i1 - 1), SLOG) + U * j) & (ps - 1);
+            const char *src = b.pool + (size_t)max(g, 0) * b.s.page_bytes + vbase +
+                              ((size_t)(t.head * (ps / U) + vs / U) * D + col) * 16;
+#pragma unroll
+            for (int d = 0; d < DT; d++) fv[d] = *reinterpret_cast<const uint4 *>(src + 256 * d);
+        };
+        auto scores = [&](float (&sc)[U]) {
+            f4_t s4[TK];
+#pragma unroll
+            for (int xx = 0; xx < TK; xx++) s4[xx] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int s = 0; s < DS; s++)
+#pragma unroll
+                for (int xx = 0; xx < TK; xx++) s4[xx] = Ops::mul(fk[xx][s], q[s], s4[xx]);
+#pragma unroll
+            for (int e = 0; e < U; e++) sc[e] = s4[e / 4][e % 4] * unscale;
+        };
+        auto sums = [&](float (&sc)[U], int base, int g) {
+            // every column sees every position of the step, or some do not
+            const bool whole = base + STEP - 1 <= p0 && (base >= low1 || base + STEP <= sinks) &&
+                               __all(g >= 0);
+            const int up = base + U * j;    // this lane's first position
+            bool odd = false;               // a value that is not finite, in a step that some rows see and others do not
+            if (!whole) {
+                uint32_t keep[U];
+#pragma unroll
+                for (int e = 0; e < U; e++) {
+                    const int p = up + e;
+                    const bool page = g >= 0;
+                    if (!(page && p <= pos && (p >= low || p < sinks))) sc[e] = -INFINITY;
+                    // what no row of the tile sees may hold anything
+                    keep[e] = page && p <= p1 && (p >= low0 || p < sinks) ? 0xffffffffu : 0u;
+                }
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    uint32_t w[4] = {fv[d].x, fv[d].y, fv[d].z, fv[d].w};
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if (U == 4) {
+                            w[i] &= keep[i];
+                            odd |= (w[i] & 0x7f800000u) == 0x7f800000u;
+                        } else {
+                            w[i] &= (keep[(2 * i) % U] & 0xffffu) | (keep[(2 * i + 1) % U] & 0xffff0000u);
+                            constexpr uint32_t X = Ops::PSHIFT != 0.0f ? 0x7c00u : 0x7f80u;
+                            odd |= (w[i] & X) == X || (w[i] & (X << 16)) == X << 16;
+                        }
+                    }
+                    fv[d] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            float mx = sc[0];
+#pragma unroll
+            for (int e = 1; e < U; e++) mx = fmaxf(mx, sc[e]);
+            mx = fmaxf(m, col_max(mx));
+            if (__any(mx > m)) {
+                const float r = __builtin_amdgcn_exp2f(m - (mx == -INFINITY ? 0.0f : mx));
+                l *= r;
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[d] *= r;
+                m = mx;
+            }
+            const float sub = (m == -INFINITY ? 0.0f : m) - Ops::PSHIFT;
+            float p[U];
+#pragma unroll
+            for (int e = 0; e < U; e++) {
+                p[e] = __builtin_amdgcn_exp2f(sc[e] - sub);
+                l += p[e];
+            }
+            const typename Ops::P pp = Ops::split(p);
+            if (p0 != p1 && __any(odd)) {
+                // column by column, each over what it sees: 0 times such a value must not reach the others
+                for (int c = 0; c < ncol; c++) {
+                    const int cp = __builtin_amdgcn_readlane(pos, c), cl = __builtin_amdgcn_readlane(low, c);
+                    uint32_t keep[U];
+#pragma unroll
+                    for (int e = 0; e < U; e++)
+                        keep[e] = up + e <= cp && (up + e >= cl || up + e < sinks) ? 0xffffffffu : 0u;
+#pragma unroll
+                    for (int d = 0; d < DT; d++) {
+                        uint32_t w[4] = {fv[d].x, fv[d].y, fv[d].z, fv[d].w};
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            w[i] &= U == 4 ? keep[i % U]
+                                           : (keep[(2 * i) % U] & 0xffffu) | (keep[(2 * i + 1) % U] & 0xffff0000u);
+                        const f4_t add = Ops::mul(make_uint4(w[0], w[1], w[2], w[3]), pp, f4_t{0.0f, 0.0f, 0.0f, 0.0f});
+                        if (col == c) o[d] += add;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[d] = Ops::mul(fv[d], pp, o[d]);
+            }
+        };
+        int i = i0 + wave;
+        if (i < i1) {
+            int gk, gv, now;
+            pages(i, gk, now);
+            load_k(i, gk);
+            load_v(i, now);
+            pages(i + AT_WAVES, gk, gv);
+            for (;;) {
+                float sc[U];
+                scores(sc);
+                __builtin_amdgcn_sched_barrier(0);
+                int gk2, gv2;
+                pages(i + 2 * AT_WAVES, gk2, gv2);
+                load_k(i + AT_WAVES, gk);
+                __builtin_amdgcn_sched_barrier(0);
+                sums(sc, kv_base(t.span, i, SLOG), now);
+                __builtin_amdgcn_sched_barrier(0);
+                load_v(i + AT_WAVES, gv);
+                now = gv;
+                gk = gk2;
+                gv = gv2;
+                if ((i += AT_WAVES) >= i1) break;
+            }
+        }
+
+        // ---- the waves together ----
+        l = col_sum(l);
+        if (j == 0) {
+            sm[wave][col] = m;
+            sl[wave][col] = l;
+        }
+#pragma unroll
+        for (int d = 0; d < DT; d++) *reinterpret_cast<f4_t *>(&so[wave][col][16 * d + 4 * j]) = o[d];
+        __syncthreads();
+        // whole: the result; else this workgroup's slot for a tile that began before it, or that goes on behind it
+        const bool mine = i0 == 0 && i1 == t.span.n;
+        float *slot = work + (size_t)(2 * blockIdx.x + (i0 == 0 ? 1 : 0)) * attn_slot(D);
+        for (int e = tid; e < ncol * (D / 4); e += AT_THREADS) {
+            const int c = e / (D / 4), d = e % (D / 4) * 4;
+            float M = sm[0][c];
+#pragma unroll
+            for (int w = 1; w < AT_WAVES; w++) M = fmaxf(M, sm[w][c]);
+            const float ms = M == -INFINITY ? 0.0f : M;
+            f4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+            float L = 0.0f;
+#pragma unroll
+            for (int w = 0; w < AT_WAVES; w++) {
+                const float r = __builtin_amdgcn_exp2f(sm[w][c] - ms);
+                sum += *reinterpret_cast<const f4_t *>(&so[w][c][d]) * r;
+                L += sl[w][c] * r;
+            }
+            if (mine) {
+                const int row = t.row0 + (c0 + c) / grp, head = t.head * grp + (c0 + c) % grp;
+                // nothing seen: L = 0 and a sum of zeros
+                const f4_t out = L == 0.0f ? sum : sum / L;
+                *reinterpret_cast<f4u_t *>(a.out + ((size_t)row * nh + head) * D + d) = out;
+            } else {
+                *reinterpret_cast<f4_t *>(slot + c * D + d) = sum;
+                if (d == 0) {
+                    slot[AT_COLS * D + c] = M;
+                    slot[AT_COLS * (D + 1) + c] = L;
+                }
+            }
+        }
+        __syncthreads();   // LDS is used again
+        x = tend;
+    }
+}
+
+// The tiles that cuts separate: workgroup (w - 1, y) takes the tile that goes
+// on over cut w if that is its first, and of its columns y, y + gridDim.y, ...
+// A thread holds a dimension, 256 / D classes of parts.
+template <int D, int SLOG>
+__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvBatch b, KvAttn a, const float *__restrict__ work,
+                                                           uint32_t most)
+{
+    extern __shared__ uint64_t pre[];
+    constexpr int CL = 256 / D;
+    __shared__ uint64_t red[4];
+    __shared__ float mx[4], part[2][CL][D];
+    at_prefix<SLOG, 256>(b, a, pre, red);
+    const uint64_t W = pre[b.n_seqs];
+    if (W == 0) return;
+    const uint32_t n = kv_parts(W, most, AT_WAVES), w = blockIdx.x + 1;
+    if (w >= n) return;
+    const AtTile t = at_find<SLOG>(b, a, pre, kv_cut(W, n, w));
+    if (t.start == kv_cut(W, n, w) || t.start < kv_cut(W, n, w - 1)) return;
+    const uint32_t w1 = kv_part(W, n, t.start + t.span.n - 1);   // the tile's parts are w - 1 .. w1
+    const int count = (int)(w1 - w) + 2;
+    const int c0 = t.t * AT_COLS, ncol = min(AT_COLS, t.rows * a.group - c0);
+    auto slot = [&](int k) { return work + (size_t)(k == 0 ? 2 * (w - 1) + 1 : 2 * (w - 1 + k)) * attn_slot(D); };
+    const int tid = threadIdx.x, d = tid % D, cl = tid / D;
+    for (int c = blockIdx.y; c < ncol; c += gridDim.y) {
+        float M = -INFINITY;
+        for (int k = tid; k < count; k += 256) M = fmaxf(M, slot(k)[AT_COLS * D + c]);
+        M = wave_max_dpp(M);
+        if ((tid & (WAVE - 1)) == 0) mx[tid / WAVE] = M;
+        __syncthreads();
+        M = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        const float ms = M == -INFINITY ? 0.0f : M;
+        float sum = 0.0f, L = 0.0f;
+        if (cl < CL)
+            for (int k = cl; k < count; k += CL) {
+                const float *s = slot(k);
+                const float r = __builtin_amdgcn_exp2f(s[AT_COLS * D + c] - ms);
+                sum = fmaf(s[c * D + d], r, sum);
+                L = fmaf(s[AT_COLS * (D + 1) + c], r, L);
+            }
+        if (cl < CL) {
+            part[0][cl][d] = sum;
+            part[1][cl][d] = L;
+        }
+        __syncthreads();
+        if (tid < D) {
+            sum = L = 0.0f;
+#pragma unroll
+            for (int k = 0; k < CL; k++) {
+                sum += part[0][k][tid];
+                L += part[1][k][tid];
+            }
+            const int row = t.row0 + (c0 + c) / a.group, head = t.head * a.group + (c0 + c) % a.group;
+            a.out[((size_t)row * a.n_heads + head) * D + tid] = L == 0.0f ? sum : sum / L;
+        }
+        __syncthreads();
+    }
 }
 
 template <class E, int D>
-__global__ __launch_bounds__(WAVE) void kv_attn_simple_kernel(KvBatch b, KvAttn a)
+static void attn_launch_d(qq_ctx *ctx, const qq_kv *kv, const KvBatch &b, const KvAttn &a)
 {
-    typedef typename E::T T;
-    constexpr int U = E::U, ND = (D + WAVE - 1) / WAVE;
-    __shared__ float ql[D];
-    __shared__ float pl[WAVE];
-    const int t = blockIdx.x, h = blockIdx.y, lane = threadIdx.x;
-    int seq, pos;
-    const bool live = kv_row(b, t, seq, pos);
-    if (!live) {
-        // a padding row gives zeros; a row of no sequence stays
-        bool own = !b.row_start;
-        for (int s = 0; !own && s < b.n_seqs; s++) {
-            int r0, r1;
-            kv_rows(b, s, r0, r1);
-            own = t >= r0 && t < r1;
-        }
-        if (own)
-            for (int d = lane; d < D; d += WAVE) a.out[((size_t)t * a.n_heads + h) * D + d] = 0.0f;
-        return;
-    }
-    const int nkv = b.s.n_kv_heads, ps = b.s.page_size, kvh = h / a.group;
-    for (int d = lane; d < D; d += WAVE) ql[d] = a.q[((size_t)t * a.n_heads + h) * D + d];
-    __syncthreads();
-    const int cap = b.stride << b.s.page_log;
-    const int hi = min(pos, cap - 1) + 1;                       // sees [0, sinks) and [lo, hi)
-    const int lo = a.window ? max(0, pos - a.window + 1) : 0;
-    const int sinks = min(a.sinks, hi);
-    float m = -INFINITY, l = 0.0f, acc[ND] = {};
-    for (int base = 0; base < hi; base += WAVE) {
-        if (base >= sinks && base + WAVE <= lo) {
-            base = (lo & ~(WAVE - 1)) - WAVE;
-            continue;
-        }
-        const int p = base + lane;
-        const int page = p < hi ? kv_page(b, seq, p) : -1;
-        const bool see = page >= 0 && (p >= lo || p < sinks);
-        float s = -INFINITY;
-        if (see) {
-            const T *k = reinterpret_cast<const T *>(b.pool + (size_t)page * b.s.page_bytes) + (size_t)kvh * ps * D;
-            float dot = 0.0f;
-            for (int c = 0; c < D / U; c++)
-                for (int e = 0; e < U; e++)
-                    dot = fmaf(ql[c * U + e], kv_to_f32(E{}, k[(c * ps + (p & (ps - 1))) * U + e]), dot);
-            s = dot * (float)a.scale;
-        }
-        const float mn = fmaxf(m, wave_maxf(s));
-        const float ms = mn == -INFINITY ? 0.0f : mn;
-        const float pr = see ? expf(s - ms) : 0.0f, f = expf(m - ms);
-        m = mn;
-        l = l * f + wave_sum(pr);
-        __syncthreads();
-        pl[lane] = see ? pr : -1.0f;   // -1: not seen
-        __syncthreads();
-        for (int j = 0; j < ND; j++) acc[j] *= f;
-        for (int j = 0; j < WAVE && base + j < hi; j++) {
-            const float w = pl[j];
-            if (w < 0.0f) continue;
-            const int g = kv_page(b, seq, base + j), slot = (base + j) & (ps - 1);
-            const T *v = reinterpret_cast<const T *>(b.pool + (size_t)g * b.s.page_bytes) + (size_t)(nkv + kvh) * ps * D;
-            for (int n = 0; n < ND; n++) {
-                const int d = n * WAVE + lane;
-                if (d < D) acc[n] = fmaf(w, kv_to_f32(E{}, v[((slot / U) * D + d) * U + slot % U]), acc[n]);
-            }
-        }
-    }
-    for (int n = 0; n < ND; n++) {
-        const int d = n * WAVE + lane;
-        if (d < D) a.out[((size_t)t * a.n_heads + h) * D + d] = l == 0.0f ? 0.0f : acc[n] / l;
-    }
+    const int parts = attn_parts(ctx);
+    const size_t shm = (size_t)(b.n_seqs + 1) * sizeof(uint64_t);
+    prof_begin(ctx, K_KV_ATTN);
+    QQ_LAUNCH(ctx, (kv_attn_kernel<E, D>), dim3(parts), dim3(AT_THREADS), shm, b, a, kv->work);
+    prof_begin(ctx, K_KV_JOIN);
+    const int cols = std::min(AT_COLS, b.row_start ? AT_COLS : a.group);
+    QQ_LAUNCH(ctx, (kv_attn_join_kernel<D, E::U == 4 ? 4 : 5>), dim3(parts - 1, cols), dim3(256), shm, b, a,
+              kv->work, (uint32_t)parts);
+    prof_end(ctx);
 }
 
 template <class E>
-static void attn_launch(qq_ctx *ctx, const KvBatch &b, const KvAttn &a)
+static void attn_launch(qq_ctx *ctx, const qq_kv *kv, const KvBatch &b, const KvAttn &a)
 {
-    const dim3 grid(b.n_rows, a.n_heads);
     switch (b.s.head_dim) {
-    case 32: QQ_LAUNCH(ctx, (kv_attn_simple_kernel<E, 32>), grid, dim3(WAVE), 0, b, a); break;
-    case 64: QQ_LAUNCH(ctx, (kv_attn_simple_kernel<E, 64>), grid, dim3(WAVE), 0, b, a); break;
-    case 96: QQ_LAUNCH(ctx, (kv_attn_simple_kernel<E, 96>), grid, dim3(WAVE), 0, b, a); break;
-    default: QQ_LAUNCH(ctx, (kv_attn_simple_kernel<E, 128>), grid, dim3(WAVE), 0, b, a); break;
+    case 32: attn_launch_d<E, 32>(ctx, kv, b, a); break;
+    case 64: attn_launch_d<E, 64>(ctx, kv, b, a); break;
+    case 96: attn_launch_d<E, 96>(ctx, kv, b, a); break;
+    default: attn_launch_d<E, 128>(ctx, kv, b, a); break;
     }
 }
 
-int launch_kv_attn(qq_ctx *ctx, const qq_kv *, const KvBatch &b, const KvAttn &a)
+int launch_kv_attn(qq_ctx *ctx, const qq_kv *kv, const KvBatch &b, const KvAttn &a)
 {
-    prof_begin(ctx, K_KV_ATTN);
-    if (b.s.type == QQ_TYPE_F32) attn_launch<KvF32>(ctx, b, a);
-    else if (b.s.type == QQ_TYPE_F16) attn_launch<KvF16>(ctx, b, a);
-    else attn_launch<KvBf16>(ctx, b, a);
-    prof_end(ctx);
+    if (b.s.type == QQ_TYPE_F32) attn_launch<KvF32>(ctx, kv, b, a);
+    else if (b.s.type == QQ_TYPE_F16) attn_launch<KvF16>(ctx, kv, b, a);
+    else attn_launch<KvBf16>(ctx, kv, b, a);
     QQ_HIP(ctx, hipGetLastError());
     return QQ_OK;
 }

@@ -305,6 +305,11 @@ int qq_kv_create(qq_ctx *ctx, void *pool_dev, size_t nbytes, int n_layers, int n
         if (e == hipSuccess) e = hipMemsetAsync(v, 0, need, ctx->stream);
         if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
     }
+    if (e == hipSuccess) {
+        void *v = nullptr;
+        e = hipMalloc(&v, kv_attn_work_bytes(ctx, s));
+        kv->work = static_cast<float *>(v);
+    }
     if (e != hipSuccess) {
         if (kv->own_pool && kv->pool) (void)hipFree(kv->pool);
         delete kv;
@@ -330,6 +335,7 @@ int qq_kv_release(qq_ctx *ctx, qq_kv *kv)
     QQ_HIP(ctx, hipSetDevice(ctx->device));
     QQ_HIP(ctx, hipStreamSynchronize(ctx->stream));
     if (kv->own_pool) (void)hipFree(kv->pool);
+    (void)hipFree(kv->work);
     delete kv;
     return QQ_OK;
 }
@@ -430,6 +436,11 @@ int qq_kv_attn_dev(qq_ctx *ctx, qq_kv *kv, int layer, const qq_kv_batch *batch, 
     if (window < 0 || sinks < 0) return set_error(ctx, "kv_attn: window %d, sinks %d", window, sinks);
     if (batch->n_seqs == 0 || batch->n_rows == 0) return QQ_OK;
     if (!q_dev || !out_dev) return set_error(ctx, "kv_attn: NULL buffer");
+    // steps of 16 positions, at the most that the tables allow: their count in 50 bits (kv_plan.h)
+    const uint64_t tiles = ((uint64_t)batch->n_rows * n_heads + 15) / 16 + (uint64_t)batch->n_seqs * kv->s.n_kv_heads;
+    if (tiles * ((uint64_t)batch->table_stride * kv->s.page_size / 16) >> 50)
+        return set_error(ctx, "kv_attn: %d rows of %d heads over tables of %d pages", batch->n_rows, n_heads,
+                         batch->table_stride);
     if (overlap(q_dev, out_dev, (size_t)batch->n_rows * n_heads * kv->s.head_dim * sizeof(float)))
         return set_error(ctx, "kv_attn: out overlaps q");
     QQ_HIP(ctx, hipSetDevice(ctx->device));

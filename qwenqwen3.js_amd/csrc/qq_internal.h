@@ -133,6 +133,7 @@ struct qq_kv {
     char *pool = nullptr;
     size_t nbytes = 0;
     bool own_pool = false;
+    float *work = nullptr;   // the attention's workspace
 };
 
 // Layers of one MoE stack (qq_moe_stack_create): borrowed layer handles, their
@@ -436,6 +437,7 @@ struct KvAttn {
     double scale;
 };
 int launch_kv_store(qq_ctx *ctx, const KvBatch &b, const KvStore &st);
+size_t kv_attn_work_bytes(const qq_ctx *ctx, const KvShape &s);
 int launch_kv_attn(qq_ctx *ctx, const qq_kv *kv, const KvBatch &b, const KvAttn &a);
 int launch_kv_copy(qq_ctx *ctx, const KvShape &s, char *pool, const int32_t *pairs, int n);
 int launch_kv_remap(qq_ctx *ctx, int32_t *table, int n, const int32_t *map, int n_map);
