@@ -25,11 +25,12 @@
 //
 // Work: all steps of the call in a row -- sequences, key/value heads, column
 // tiles, each tile's span -- are cut into equal parts, one a workgroup,
-// wherever the cuts fall (kv_plan.h); lengths are read on the device.  A
-// workgroup's waves take its steps in turn and join in LDS; what a cut
-// separates goes to the workspace, two slots a workgroup (a tile it goes on
-// with from the workgroup before it, and one it leaves to the next), and a
-// second launch joins those.
+// wherever the cuts fall (kv_plan.h); lengths are read on the device.  A tile
+// counts AT_LEAD steps more than it has, ahead of its own: what its query,
+// its first loads and its end cost a workgroup.  A workgroup's waves take its
+// steps in turn and join in LDS; what a cut separates goes to the workspace,
+// two slots a workgroup (a tile it goes on with from the workgroup before it,
+// and one it leaves to the next), and a second launch joins those.
 #include "kv_device.h"
 #include "kv_plan.h"
 
@@ -43,14 +44,24 @@ typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 constexpr int AT_COLS = 16;      // columns of a tile
 constexpr int AT_WAVES = 4;      // waves of a workgroup
 constexpr int AT_THREADS = AT_WAVES * WAVE;
-constexpr int AT_PER_CU = 2;     // workgroups a CU holds
+constexpr int AT_LEAD = 4;       // steps that a tile's beginning and end are worth
+constexpr int AT_LEAST = 4;      // steps a part has at least
+// workgroups a CU holds, by registers: a wave keeps two steps of values and one of keys, q's planes and the sums
+__host__ __device__ constexpr int at_per_cu(int dim) { return dim == 32 ? 4 : dim == 64 ? 3 : 2; }
 
-static int attn_parts(const qq_ctx *ctx) { return std::min(ctx->num_cus * AT_PER_CU, 4095); }
-// floats of a workspace slot: 16 columns of D sums, their maxima and sums of probabilities
+static int attn_parts(const qq_ctx *ctx, int dim) { return std::min(ctx->num_cus * at_per_cu(dim), 4095); }
+// The workspace: what every workgroup leaves to the join (count 0: nothing),
+// then its slots, in floats: 16 columns of D sums, their maxima and sums of
+// probabilities.
+struct AtJoin {
+    int count;                   // workgroups that share the tile, this one the first
+    int row0, c0, ncol, head;    // its sequence's first row, its columns, its key/value head
+    int pad[3];
+};
 __host__ __device__ constexpr int attn_slot(int dim) { return AT_COLS * (dim + 2); }
 size_t kv_attn_work_bytes(const qq_ctx *ctx, const KvShape &s)
 {
-    return (size_t)attn_parts(ctx) * 2 * attn_slot(s.head_dim) * sizeof(float);
+    return (size_t)attn_parts(ctx, s.head_dim) * (sizeof(AtJoin) + 2 * attn_slot(s.head_dim) * sizeof(float));
 }
 
 // ---- operands by cache type: q's planes, a step's probabilities -------------------
@@ -155,12 +166,22 @@ __device__ __forceinline__ float col_sum(float v)
     return f_of(b[0]) + f_of(b[1]);
 }
 
+// 16 bytes of the pool; ONCE: that this call reads once.
+template <bool ONCE>
+__device__ __forceinline__ uint4 at_load(const char *p)
+{
+    typedef unsigned int v4u __attribute__((ext_vector_type(4)));
+    if (!ONCE) return *reinterpret_cast<const uint4 *>(p);
+    const v4u v = __builtin_nontemporal_load(reinterpret_cast<const v4u *>(p));
+    return make_uint4(v.x, v.y, v.z, v.w);
+}
+
 // ---- the plan, in every workgroup ---------------------------------------------------
 
 struct AtTile {
     int seq, head, t;        // sequence, key/value head, column tile
     int row0, rows, len;     // the sequence's new rows and length
-    uint64_t start;          // the tile's first step among the call's
+    uint64_t start;          // the tile's first step among the call's (AT_LEAD of them ahead of its own)
     KvSpan span;
 };
 
@@ -182,7 +203,7 @@ __device__ __forceinline__ void at_prefix(const KvBatch &b, const KvAttn &a, uin
         kv_rows(b, s, r0, r1);
         const int len = max(b.len[s], 0), n = kv_tiles(r1 - r0, a.group, AT_COLS);
         uint64_t steps = 0;
-        for (int t = 0; t < n; t++) steps += at_span<SLOG>(b, a, len, r1 - r0, t).n;
+        for (int t = 0; t < n; t++) steps += at_span<SLOG>(b, a, len, r1 - r0, t).n + AT_LEAD;
         pre[s] = sum;      // within this thread's run
         sum += steps * b.s.n_kv_heads;
     }
@@ -222,15 +243,17 @@ __device__ __forceinline__ AtTile at_find(const KvBatch &b, const KvAttn &a, con
     t.start = pre[lo] + per * t.head;
     for (t.t = 0;; t.t++) {
         t.span = at_span<SLOG>(b, a, t.len, t.rows, t.t);
-        if (x < t.start + t.span.n) return t;
-        t.start += t.span.n;
+        if (x < t.start + AT_LEAD + t.span.n) return t;
+        t.start += AT_LEAD + t.span.n;
     }
 }
 
 // ---- the kernel ---------------------------------------------------------------------
 
-template <class E, int D>
-__global__ __launch_bounds__(AT_THREADS, AT_PER_CU) void kv_attn_kernel(KvBatch b, KvAttn a, float *__restrict__ work)
+// ROWS: a tile's columns may be several rows, that see different positions.
+template <class E, int D, bool ROWS>
+__global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBatch b, KvAttn a,
+                                                                          AtJoin *__restrict__ joins)
 {
     typedef AtOps<E> Ops;
     constexpr int U = E::U, TK = U / 4, DS = D / (4 * U), DT = D / 16;
@@ -241,12 +264,13 @@ __global__ __launch_bounds__(AT_THREADS, AT_PER_CU) void kv_attn_kernel(KvBatch 
     __shared__ float sm[AT_WAVES][AT_COLS], sl[AT_WAVES][AT_COLS];
     __shared__ uint64_t red[AT_WAVES];
     at_prefix<SLOG, AT_THREADS>(b, a, pre, red);
+    float *const work = reinterpret_cast<float *>(joins + gridDim.x);
     const uint64_t W = pre[b.n_seqs];
-    if (W == 0) return;
-    const uint32_t n = kv_parts(W, gridDim.x, AT_WAVES);
-    if (blockIdx.x >= n) return;
-    const uint64_t x1 = kv_cut(W, n, blockIdx.x + 1);
-    const uint64_t x0 = kv_cut(W, n, blockIdx.x);
+    const uint32_t n = kv_parts(W, gridDim.x, AT_LEAST);
+    // (no steps, or fewer parts than workgroups: none for this one)
+    const uint64_t x0 = W && blockIdx.x < n ? kv_cut(W, n, blockIdx.x) : 0;
+    const uint64_t x1 = W && blockIdx.x < n ? kv_cut(W, n, blockIdx.x + 1) : 0;
+    int left_count = 0, left_row0 = 0, left_c0 = 0, left_ncol = 0, left_head = 0;   // this workgroup's AtJoin
 
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
     const int col = lane & 15, j = lane >> 4;
@@ -258,91 +282,54 @@ __global__ __launch_bounds__(AT_THREADS, AT_PER_CU) void kv_attn_kernel(KvBatch 
 
     for (uint64_t x = x0; x < x1;) {
         const AtTile t = at_find<SLOG>(b, a, pre, x);
-        const int i0 = (int)(x - t.start);
-        const uint64_t tend = t.start + t.span.n;
-        const int i1 = (int)((tend < x1 ? tend : x1) - t.start);
+        const uint64_t own = t.start + AT_LEAD, tend = own + t.span.n;
+        x = tend;
+        if (own >= x1) break;    // the next workgroup's
+        const int i0 = x0 > own ? (int)(x0 - own) : 0;
+        const int i1 = (int)((tend < x1 ? tend : x1) - own);
         const int c0 = t.t * AT_COLS, ncol = min(AT_COLS, t.rows * grp - c0);
         // rows of the tile's columns, and their positions
         const int p0 = t.len - t.rows + c0 / grp, p1 = t.len - t.rows + (c0 + ncol - 1) / grp;
-        const int cr = (c0 + col) / grp;
-        const bool live = col < ncol;
-        const int pos = live ? t.len - t.rows + cr : -1;
+        // columns behind the tile's last do what that one does, and are not stored
+        const int cc = c0 + min(col, ncol - 1), cr = cc / grp;
+        const int pos = t.len - t.rows + cr;
         const int low = a.window && pos >= 0 ? max(pos - a.window + 1, 0) : 0;
         const int low0 = a.window && p0 >= 0 ? max(p0 - a.window + 1, 0) : 0;   // what the tile's first ...
         const int low1 = a.window && p1 >= 0 ? max(p1 - a.window + 1, 0) : 0;   // ... and last row's windows start with
         const int sinks = a.sinks;
-
-        // ---- q in planes ----
-        typename Ops::Q q[DS];
-        float unscale = 1.0f;
-        {
-            float v[DS][U];
-            const float *src = a.q + ((size_t)(t.row0 + cr) * nh + t.head * grp + (c0 + col) % grp) * D;
-            float big = 0.0f;
-#pragma unroll
-            for (int s = 0; s < DS; s++)
-#pragma unroll
-                for (int e = 0; e < U; e++) {
-                    v[s][e] = live ? src[(4 * s + j) * U + e] * qscale : 0.0f;
-                    big = fmaxf(big, fabsf(v[s][e]));
-                }
-            if (Ops::PSHIFT != 0.0f) {
-                // the largest to [2^14, 2^15)
-                const int f = min(268 - (int)(__float_as_uint(col_max(big)) >> 23), 253);
-                unscale = __uint_as_float((uint32_t)(254 - f) << 23);
-                const float up = __uint_as_float((uint32_t)f << 23);
-#pragma unroll
-                for (int s = 0; s < DS; s++)
-#pragma unroll
-                    for (int e = 0; e < U; e++) v[s][e] *= up;
-            }
-#pragma unroll
-            for (int s = 0; s < DS; s++) q[s] = Ops::split(v[s]);
-        }
 
         float m = -INFINITY, l = 0.0f;
         f4_t o[DT];
 #pragma unroll
         for (int d = 0; d < DT; d++) o[d] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
 
-        // One step's operands in registers.  Keys are loaded for the next step
-        // once this step's scores are formed, values once its sums are: each
-        // has the other half of a step to arrive in.  (Table entries are read
-        // a step ahead of the loads that need them.)
-        uint4 fk[TK][DS], fv[DT];
-        auto pages = [&](int i, int &gk, int &gv) {
+        // Keys and values of the next step are loaded once this step's scores
+        // are formed: a step is in flight all the time.  (Table entries are
+        // read a step ahead of the loads that need them.)
+        uint4 fk[TK][DS], fva[DT], fvb[DT];
+        auto entries = [&](int i, int &gk, int &gv) {
             const int base = kv_base(t.span, min(i, i1 - 1), SLOG);
-            gk = kv_page(b, t.seq, base + U * ku);
-            gv = kv_page(b, t.seq, base + U * j);
+            gk = kv_entry(b, t.seq, base + U * ku);
+            gv = kv_entry(b, t.seq, base + U * j);
         };
         auto load_k = [&](int i, int g) {
-            const int ks = (kv_base(t.span, min(i, i1 - 1), SLOG) + kp) & (ps - 1);
-            const char *src = b.pool + (size_t)max(g, 0) * b.s.page_bytes + ((size_t)(t.head * (D / U) + j) * ps + ks) * 16;
+            const int at = kv_base(t.span, min(i, i1 - 1), SLOG) + kp, ks = at & (ps - 1);
+            const char *src = b.pool + (size_t)max(kv_page_of(b, at, g), 0) * b.s.page_bytes + ((size_t)(t.head * (D / U) + j) * ps + ks) * 16;
 #pragma unroll
             for (int s = 0; s < DS; s++)
 #pragma unroll
                 for (int xx = 0; xx < TK; xx++)
-                    fk[xx][s] = *reinterpret_cast<const uint4 *>(src + (size_t)s * 64 * ps + 64 * xx);
+                    fk[xx][s] = at_load<!ROWS>(src + (size_t)s * 64 * ps + 64 * xx);
         };
-        auto load_v = [&](int i, int g) {
-            const int vs = (kv_base(t.span, min(i, i1 - 1), SLOG) + U * j) & (ps - 1);
-            const char *src = b.pool + (size_t)max(g, 0) * b.s.page_bytes + vbase +
+        auto load_v = [&](uint4 (&fv)[DT], int i, int g) {
+            const int at = kv_base(t.span, min(i, i1 - 1), SLOG) + U * j, vs = at & (ps - 1);
+            const char *src = b.pool + (size_t)max(kv_page_of(b, at, g), 0) * b.s.page_bytes + vbase +
                               ((size_t)(t.head * (ps / U) + vs / U) * D + col) * 16;
 #pragma unroll
-            for (int d = 0; d < DT; d++) fv[d] = *reinterpret_cast<const uint4 *>(src + 256 * d);
+            for (int d = 0; d < DT; d++) fv[d] = at_load<!ROWS>(src + 256 * d);
         };
-        auto scores = [&](float (&sc)[U]) {
-            f4_t s4[TK];
-#pragma unroll
-            for (int xx = 0; xx < TK; xx++) s4[xx] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int s = 0; s < DS; s++)
-#pragma unroll
-                for (int xx = 0; xx < TK; xx++) s4[xx] = Ops::mul(fk[xx][s], q[s], s4[xx]);
-#pragma unroll
-            for (int e = 0; e < U; e++) sc[e] = s4[e / 4][e % 4] * unscale;
-        };
-        auto sums = [&](float (&sc)[U], int base, int g) {
+        auto sums = [&](uint4 (&fv)[DT], float (&sc)[U], int base, int entry) {
+            const int g = kv_page_of(b, base + U * j, entry);
             // every column sees every position of the step, or some do not
             const bool whole = base + STEP - 1 <= p0 && (base >= low1 || base + STEP <= sinks) &&
                                __all(g >= 0);
@@ -365,11 +352,11 @@ __global__ __launch_bounds__(AT_THREADS, AT_PER_CU) void kv_attn_kernel(KvBatch 
                     for (int i = 0; i < 4; i++) {
                         if (U == 4) {
                             w[i] &= keep[i];
-                            odd |= (w[i] & 0x7f800000u) == 0x7f800000u;
+                            if (ROWS) odd |= (w[i] & 0x7f800000u) == 0x7f800000u;
                         } else {
                             w[i] &= (keep[(2 * i) % U] & 0xffffu) | (keep[(2 * i + 1) % U] & 0xffff0000u);
                             constexpr uint32_t X = Ops::PSHIFT != 0.0f ? 0x7c00u : 0x7f80u;
-                            odd |= (w[i] & X) == X || (w[i] & (X << 16)) == X << 16;
+                            if (ROWS) odd |= (w[i] & X) == X || (w[i] & (X << 16)) == X << 16;
                         }
                     }
                     fv[d] = make_uint4(w[0], w[1], w[2], w[3]);
@@ -394,7 +381,7 @@ __global__ __launch_bounds__(AT_THREADS, AT_PER_CU) void kv_attn_kernel(KvBatch 
                 l += p[e];
             }
             const typename Ops::P pp = Ops::split(p);
-            if (p0 != p1 && __any(odd)) {
+            if (ROWS && p0 != p1 && __any(odd)) {
                 // column by column, each over what it sees: 0 times such a value must not reach the others
                 for (int c = 0; c < ncol; c++) {
                     const int cp = __builtin_amdgcn_readlane(pos, c), cl = __builtin_amdgcn_readlane(low, c);
@@ -410,7 +397,8 @@ __global__ __launch_bounds__(AT_THREADS, AT_PER_CU) void kv_attn_kernel(KvBatch 
                             w[i] &= U == 4 ? keep[i % U]
                                            : (keep[(2 * i) % U] & 0xffffu) | (keep[(2 * i + 1) % U] & 0xffff0000u);
                         const f4_t add = Ops::mul(make_uint4(w[0], w[1], w[2], w[3]), pp, f4_t{0.0f, 0.0f, 0.0f, 0.0f});
-                        if (col == c) o[d] += add;
+                        #pragma unroll
+                        for (int r = 0; r < 4; r++) o[d][r] += col == c ? add[r] : 0.0f;
                     }
                 }
             } else {
@@ -418,29 +406,80 @@ __global__ __launch_bounds__(AT_THREADS, AT_PER_CU) void kv_attn_kernel(KvBatch 
                 for (int d = 0; d < DT; d++) o[d] = Ops::mul(fv[d], pp, o[d]);
             }
         };
+        // ---- the first loads, then q in planes ----
         int i = i0 + wave;
-        if (i < i1) {
-            int gk, gv, now;
-            pages(i, gk, now);
-            load_k(i, gk);
-            load_v(i, now);
-            pages(i + AT_WAVES, gk, gv);
-            for (;;) {
-                float sc[U];
-                scores(sc);
-                __builtin_amdgcn_sched_barrier(0);
-                int gk2, gv2;
-                pages(i + 2 * AT_WAVES, gk2, gv2);
-                load_k(i + AT_WAVES, gk);
-                __builtin_amdgcn_sched_barrier(0);
-                sums(sc, kv_base(t.span, i, SLOG), now);
-                __builtin_amdgcn_sched_barrier(0);
-                load_v(i + AT_WAVES, gv);
-                now = gv;
-                gk = gk2;
-                gv = gv2;
-                if ((i += AT_WAVES) >= i1) break;
+        int gk, gv, now, gk1, gv1;
+        entries(i, gk, now);
+        entries(i + AT_WAVES, gk1, gv1);
+        typename Ops::Q q[DS];
+        float unscale = 1.0f;
+        {
+            f4_t v[DS][U / 4];
+            const float *src = a.q + ((size_t)(t.row0 + cr) * nh + t.head * grp + cc % grp) * D + j * U;
+#pragma unroll
+            for (int s = 0; s < DS; s++)
+#pragma unroll
+                for (int e = 0; e < U / 4; e++) v[s][e] = *reinterpret_cast<const f4u_t *>(src + 4 * U * s + 4 * e);
+            if (i < i1) {
+                load_k(i, gk);
+                load_v(fva, i, now);
             }
+            gk = gk1;
+            gv = gv1;
+            __builtin_amdgcn_sched_barrier(0);
+            float up = qscale;
+            if (Ops::PSHIFT != 0.0f) {
+                // the largest to [2^14, 2^15)
+                float big = 0.0f;
+#pragma unroll
+                for (int s = 0; s < DS; s++)
+#pragma unroll
+                    for (int e = 0; e < U; e++) big = fmaxf(big, fabsf(v[s][e / 4][e % 4] * qscale));
+                const int f = min(268 - (int)(__float_as_uint(col_max(big)) >> 23), 253);
+                unscale = __uint_as_float((uint32_t)(254 - f) << 23);
+                up = __uint_as_float((uint32_t)f << 23);
+            }
+#pragma unroll
+            for (int s = 0; s < DS; s++) {
+                float x[U];
+#pragma unroll
+                for (int e = 0; e < U; e++)
+                    x[e] = Ops::PSHIFT != 0.0f ? v[s][e / 4][e % 4] * qscale * up : v[s][e / 4][e % 4] * qscale;
+                q[s] = Ops::split(x);
+            }
+        }
+
+        auto scores = [&](float (&sc)[U]) {
+            f4_t s4[TK];
+#pragma unroll
+            for (int xx = 0; xx < TK; xx++) s4[xx] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int s = 0; s < DS; s++)
+#pragma unroll
+                for (int xx = 0; xx < TK; xx++) s4[xx] = Ops::mul(fk[xx][s], q[s], s4[xx]);
+#pragma unroll
+            for (int e = 0; e < U; e++) sc[e] = s4[e / 4][e % 4] * unscale;
+        };
+        auto step = [&](uint4 (&cur)[DT], uint4 (&next)[DT]) {
+            float sc[U];
+            scores(sc);
+            __builtin_amdgcn_sched_barrier(0);
+            if (i + AT_WAVES < i1) {
+                load_k(i + AT_WAVES, gk);
+                load_v(next, i + AT_WAVES, gv);
+            }
+            entries(i + 2 * AT_WAVES, gk, gv1);
+            __builtin_amdgcn_sched_barrier(0);
+            sums(cur, sc, kv_base(t.span, i, SLOG), now);
+            __builtin_amdgcn_sched_barrier(0);
+            now = gv;
+            gv = gv1;
+            i += AT_WAVES;
+        };
+        while (i < i1) {
+            step(fva, fvb);
+            if (i >= i1) break;
+            step(fvb, fva);
         }
 
         // ---- the waves together ----
@@ -482,80 +521,102 @@ __global__ __launch_bounds__(AT_THREADS, AT_PER_CU) void kv_attn_kernel(KvBatch 
                 }
             }
         }
+        if (i0 == 0 && !mine) {
+            left_count = (int)(kv_part(W, n, tend - 1) - blockIdx.x) + 1;
+            left_row0 = t.row0;
+            left_c0 = c0;
+            left_ncol = ncol;
+            left_head = t.head;
+        }
         __syncthreads();   // LDS is used again
-        x = tend;
     }
+    if (tid == 0) joins[blockIdx.x] = AtJoin{left_count, left_row0, left_c0, left_ncol, left_head, {0, 0, 0}};
 }
 
-// The tiles that cuts separate: workgroup (w - 1, y) takes the tile that goes
-// on over cut w if that is its first, and of its columns y, y + gridDim.y, ...
-// A thread holds a dimension, 256 / D classes of parts.
-template <int D, int SLOG>
-__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvBatch b, KvAttn a, const float *__restrict__ work,
-                                                           uint32_t most)
+// The tiles that cuts separate: workgroup (w, c) takes column c of the tile
+// that part w leaves to those behind it.  A thread holds four dimensions, and
+// 256 / (D / 4) classes of parts their running maximum and sums.
+template <int D>
+__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttn a, const AtJoin *__restrict__ joins)
 {
-    extern __shared__ uint64_t pre[];
-    constexpr int CL = 256 / D;
-    __shared__ uint64_t red[4];
-    __shared__ float mx[4], part[2][CL][D];
-    at_prefix<SLOG, 256>(b, a, pre, red);
-    const uint64_t W = pre[b.n_seqs];
-    if (W == 0) return;
-    const uint32_t n = kv_parts(W, most, AT_WAVES), w = blockIdx.x + 1;
-    if (w >= n) return;
-    const AtTile t = at_find<SLOG>(b, a, pre, kv_cut(W, n, w));
-    if (t.start == kv_cut(W, n, w) || t.start < kv_cut(W, n, w - 1)) return;
-    const uint32_t w1 = kv_part(W, n, t.start + t.span.n - 1);   // the tile's parts are w - 1 .. w1
-    const int count = (int)(w1 - w) + 2;
-    const int c0 = t.t * AT_COLS, ncol = min(AT_COLS, t.rows * a.group - c0);
-    auto slot = [&](int k) { return work + (size_t)(k == 0 ? 2 * (w - 1) + 1 : 2 * (w - 1 + k)) * attn_slot(D); };
-    const int tid = threadIdx.x, d = tid % D, cl = tid / D;
-    for (int c = blockIdx.y; c < ncol; c += gridDim.y) {
-        float M = -INFINITY;
-        for (int k = tid; k < count; k += 256) M = fmaxf(M, slot(k)[AT_COLS * D + c]);
-        M = wave_max_dpp(M);
-        if ((tid & (WAVE - 1)) == 0) mx[tid / WAVE] = M;
-        __syncthreads();
-        M = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        const float ms = M == -INFINITY ? 0.0f : M;
-        float sum = 0.0f, L = 0.0f;
-        if (cl < CL)
-            for (int k = cl; k < count; k += CL) {
-                const float *s = slot(k);
-                const float r = __builtin_amdgcn_exp2f(s[AT_COLS * D + c] - ms);
-                sum = fmaf(s[c * D + d], r, sum);
-                L = fmaf(s[AT_COLS * (D + 1) + c], r, L);
-            }
-        if (cl < CL) {
-            part[0][cl][d] = sum;
-            part[1][cl][d] = L;
-        }
-        __syncthreads();
-        if (tid < D) {
-            sum = L = 0.0f;
+    constexpr int LN = D / 4, CL = 256 / LN, AHEAD = 8;
+    __shared__ float sm[CL], sl[CL];
+    __shared__ __align__(16) f4_t so[CL][LN];
+    const AtJoin t = joins[blockIdx.x];
+    const int c = blockIdx.y;
+    if (c >= t.ncol || t.count == 0) return;
+    const float *work = reinterpret_cast<const float *>(joins + gridDim.x);
+    const int cl = threadIdx.x / LN, ln = threadIdx.x % LN;
+    float M = -INFINITY, L = 0.0f;
+    f4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (cl < CL)
+        for (int k0 = cl; k0 < t.count; k0 += AHEAD * CL) {
+            float m[AHEAD], l[AHEAD];
+            f4_t o[AHEAD];
 #pragma unroll
-            for (int k = 0; k < CL; k++) {
-                sum += part[0][k][tid];
-                L += part[1][k][tid];
+            for (int u = 0; u < AHEAD; u++) {
+                const int k = min(k0 + u * CL, t.count - 1);
+                const float *s = work + (size_t)(2 * (blockIdx.x + k) + (k == 0)) * attn_slot(D);
+                m[u] = s[AT_COLS * D + c];
+                l[u] = s[AT_COLS * (D + 1) + c];
+                o[u] = *reinterpret_cast<const f4_t *>(s + c * D + 4 * ln);
             }
-            const int row = t.row0 + (c0 + c) / a.group, head = t.head * a.group + (c0 + c) % a.group;
-            a.out[((size_t)row * a.n_heads + head) * D + tid] = L == 0.0f ? sum : sum / L;
+            float top = M;
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++)
+                if (k0 + u * CL < t.count) top = fmaxf(top, m[u]);
+            const float ms = top == -INFINITY ? 0.0f : top;
+            const float r = __builtin_amdgcn_exp2f(M - ms);
+            sum *= r;
+            L *= r;
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++)
+                if (k0 + u * CL < t.count) {
+                    const float w = __builtin_amdgcn_exp2f(m[u] - ms);
+                    sum += o[u] * w;
+                    L += l[u] * w;
+                }
+            M = top;
         }
-        __syncthreads();
+    if (cl < CL) {
+        so[cl][ln] = sum;
+        if (ln == 0) {
+            sm[cl] = M;
+            sl[cl] = L;
+        }
     }
+    __syncthreads();
+    if (threadIdx.x >= LN) return;
+    const int top = min(CL, t.count);
+    M = sm[0];
+    for (int k = 1; k < top; k++) M = fmaxf(M, sm[k]);
+    const float ms = M == -INFINITY ? 0.0f : M;
+    sum = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    L = 0.0f;
+    for (int k = 0; k < top; k++) {
+        const float w = __builtin_amdgcn_exp2f(sm[k] - ms);
+        sum += so[k][ln] * w;
+        L += sl[k] * w;
+    }
+    const int row = t.row0 + (t.c0 + c) / a.group, head = t.head * a.group + (t.c0 + c) % a.group;
+    const f4_t out = L == 0.0f ? sum : sum / L;
+    *reinterpret_cast<f4u_t *>(a.out + ((size_t)row * a.n_heads + head) * D + 4 * ln) = out;
 }
 
 template <class E, int D>
 static void attn_launch_d(qq_ctx *ctx, const qq_kv *kv, const KvBatch &b, const KvAttn &a)
 {
-    const int parts = attn_parts(ctx);
+    const int parts = attn_parts(ctx, D);
     const size_t shm = (size_t)(b.n_seqs + 1) * sizeof(uint64_t);
+    AtJoin *joins = reinterpret_cast<AtJoin *>(kv->work);
     prof_begin(ctx, K_KV_ATTN);
-    QQ_LAUNCH(ctx, (kv_attn_kernel<E, D>), dim3(parts), dim3(AT_THREADS), shm, b, a, kv->work);
+    if (b.row_start)
+        QQ_LAUNCH(ctx, (kv_attn_kernel<E, D, true>), dim3(parts), dim3(AT_THREADS), shm, b, a, joins);
+    else
+        QQ_LAUNCH(ctx, (kv_attn_kernel<E, D, false>), dim3(parts), dim3(AT_THREADS), shm, b, a, joins);
     prof_begin(ctx, K_KV_JOIN);
     const int cols = std::min(AT_COLS, b.row_start ? AT_COLS : a.group);
-    QQ_LAUNCH(ctx, (kv_attn_join_kernel<D, E::U == 4 ? 4 : 5>), dim3(parts - 1, cols), dim3(256), shm, b, a,
-              kv->work, (uint32_t)parts);
+    QQ_LAUNCH(ctx, kv_attn_join_kernel<D>, dim3(parts, cols), dim3(256), 0, a, joins);
     prof_end(ctx);
 }
 

@@ -66,13 +66,20 @@ __device__ __forceinline__ bool kv_row(const KvBatch &b, int t, int &seq, int &p
     return pos >= 0;
 }
 
-// The page of position pos >= 0 of a sequence, -1 when it has none.
+// The table's entry for position pos >= 0 of a sequence, read without a
+// condition (a load under a branch is waited for where the branch ends, and
+// everything in flight with it), and the page that it is, -1 for none.
+__device__ __forceinline__ int kv_entry(const KvBatch &b, int seq, int pos)
+{
+    return b.table[(size_t)seq * b.stride + min(pos >> b.s.page_log, b.stride - 1)];
+}
+__device__ __forceinline__ int kv_page_of(const KvBatch &b, int pos, int entry)
+{
+    return (pos >> b.s.page_log) < b.stride && (unsigned)entry < (unsigned)b.s.n_pages ? entry : -1;
+}
 __device__ __forceinline__ int kv_page(const KvBatch &b, int seq, int pos)
 {
-    const int i = pos >> b.s.page_log;
-    if (i >= b.stride) return -1;
-    const int g = b.table[(size_t)seq * b.stride + i];
-    return (unsigned)g < (unsigned)b.s.n_pages ? g : -1;
+    return kv_page_of(b, pos, kv_entry(b, seq, pos));
 }
 
 }  // namespace qq
