@@ -34,10 +34,13 @@
 #include "kv_device.h"
 #include "kv_plan.h"
 
+#include <type_traits>
+
 namespace qq {
 
 typedef float f4_t __attribute__((ext_vector_type(4)));
 typedef float f4u_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f16_t __attribute__((ext_vector_type(16)));
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 h8_t __attribute__((ext_vector_type(8)));
 
@@ -50,18 +53,25 @@ constexpr int AT_LEAST = 4;      // steps a part has at least
 __host__ __device__ constexpr int at_per_cu(int dim) { return dim == 32 ? 4 : dim == 64 ? 3 : 2; }
 
 static int attn_parts(const qq_ctx *ctx, int dim) { return std::min(ctx->num_cus * at_per_cu(dim), 4095); }
+// The form for many rows: 128 columns, 32 a wave
+constexpr int AW_COLS = 128;
+constexpr int AW_PER_CU = 2;
+static int wide_parts(const qq_ctx *ctx) { return std::min(ctx->num_cus * AW_PER_CU, 4095); }
+
 // The workspace: what every workgroup leaves to the join (count 0: nothing),
-// then its slots, in floats: 16 columns of D sums, their maxima and sums of
+// then its slots, in floats: the columns' D sums, their maxima and sums of
 // probabilities.
 struct AtJoin {
     int count;                   // workgroups that share the tile, this one the first
     int row0, c0, ncol, head;    // its sequence's first row, its columns, its key/value head
     int pad[3];
 };
-__host__ __device__ constexpr int attn_slot(int dim) { return AT_COLS * (dim + 2); }
+__host__ __device__ constexpr int attn_slot(int cols, int dim) { return cols * (dim + 2); }
 size_t kv_attn_work_bytes(const qq_ctx *ctx, const KvShape &s)
 {
-    return (size_t)attn_parts(ctx, s.head_dim) * (sizeof(AtJoin) + 2 * attn_slot(s.head_dim) * sizeof(float));
+    const size_t narrow = sizeof(AtJoin) + 2 * attn_slot(AT_COLS, s.head_dim) * sizeof(float);
+    const size_t wide = sizeof(AtJoin) + 2 * attn_slot(AW_COLS, s.head_dim) * sizeof(float);
+    return std::max(attn_parts(ctx, s.head_dim) * narrow, wide_parts(ctx) * wide);
 }
 
 // ---- operands by cache type: q's planes, a step's probabilities -------------------
@@ -80,6 +90,13 @@ struct AtOps {
         const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
         for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w[i]), q.v[i], c, 0, 0, 0);
+        return c;
+    }
+    static __device__ __forceinline__ f16_t mul(const uint4 &a, const Q &q, f16_t c)
+    {
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(w[i]), q.v[i], c, 0, 0, 0);
         return c;
     }
 };
@@ -119,6 +136,13 @@ struct AtOps<KvBf16> {
         c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, q.m, c, 0, 0, 0);
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, q.h, c, 0, 0, 0);
     }
+    static __device__ __forceinline__ f16_t mul(const uint4 &a, const Q &q, f16_t c)
+    {
+        const b8_t v = __builtin_bit_cast(b8_t, a);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, q.l, c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, q.m, c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, q.h, c, 0, 0, 0);
+    }
 };
 
 template <>
@@ -144,6 +168,12 @@ struct AtOps<KvF16> {
         c = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, q.l, c, 0, 0, 0);
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(v, q.h, c, 0, 0, 0);
     }
+    static __device__ __forceinline__ f16_t mul(const uint4 &a, const Q &q, f16_t c)
+    {
+        const h8_t v = __builtin_bit_cast(h8_t, a);
+        c = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, q.l, c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(v, q.h, c, 0, 0, 0);
+    }
 };
 
 // ---- lanes ------------------------------------------------------------------------
@@ -166,6 +196,14 @@ __device__ __forceinline__ float col_sum(float v)
     return f_of(b[0]) + f_of(b[1]);
 }
 
+// A value from its bits.
+__device__ __forceinline__ float at_value(KvF32, uint32_t b) { return __uint_as_float(b); }
+template <class E>
+__device__ __forceinline__ float at_value(E e, uint32_t b)
+{
+    return kv_to_f32(e, (uint16_t)b);
+}
+
 // 16 bytes of the pool; ONCE: that this call reads once.
 template <bool ONCE>
 __device__ __forceinline__ uint4 at_load(const char *p)
@@ -174,6 +212,18 @@ __device__ __forceinline__ uint4 at_load(const char *p)
     if (!ONCE) return *reinterpret_cast<const uint4 *>(p);
     const v4u v = __builtin_nontemporal_load(reinterpret_cast<const v4u *>(p));
     return make_uint4(v.x, v.y, v.z, v.w);
+}
+
+// The same over the two lanes of one column (l, l ^ 32).
+__device__ __forceinline__ float half_max(float v)
+{
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(f_of(b[0]), f_of(b[1]));
+}
+__device__ __forceinline__ float half_sum(float v)
+{
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return f_of(b[0]) + f_of(b[1]);
 }
 
 // ---- the plan, in every workgroup ---------------------------------------------------
@@ -185,14 +235,14 @@ struct AtTile {
     KvSpan span;
 };
 
-template <int SLOG>
+template <int COLS, int SLOG>
 __device__ __forceinline__ KvSpan at_span(const KvBatch &b, const KvAttn &a, int len, int rows, int t)
 {
-    return kv_tile_span(len, rows, t, AT_COLS, a.group, b.stride << b.s.page_log, a.window, a.sinks, SLOG);
+    return kv_tile_span(len, rows, t, COLS, a.group, b.stride << b.s.page_log, a.window, a.sinks, SLOG);
 }
 
 // pre[i] = steps of the sequences ahead of i, for i <= n_seqs (threads: the whole workgroup).
-template <int SLOG, int NT>
+template <int COLS, int SLOG, int NT>
 __device__ __forceinline__ void at_prefix(const KvBatch &b, const KvAttn &a, uint64_t *pre, uint64_t *red)
 {
     const int per = (b.n_seqs + NT - 1) / NT, tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
@@ -201,9 +251,9 @@ __device__ __forceinline__ void at_prefix(const KvBatch &b, const KvAttn &a, uin
     for (int s = s0; s < s1; s++) {
         int r0, r1;
         kv_rows(b, s, r0, r1);
-        const int len = max(b.len[s], 0), n = kv_tiles(r1 - r0, a.group, AT_COLS);
+        const int len = max(b.len[s], 0), n = kv_tiles(r1 - r0, a.group, COLS);
         uint64_t steps = 0;
-        for (int t = 0; t < n; t++) steps += at_span<SLOG>(b, a, len, r1 - r0, t).n + AT_LEAD;
+        for (int t = 0; t < n; t++) steps += at_span<COLS, SLOG>(b, a, len, r1 - r0, t).n + AT_LEAD;
         pre[s] = sum;      // within this thread's run
         sum += steps * b.s.n_kv_heads;
     }
@@ -223,7 +273,7 @@ __device__ __forceinline__ void at_prefix(const KvBatch &b, const KvAttn &a, uin
 }
 
 // The tile that holds step x.
-template <int SLOG>
+template <int COLS, int SLOG>
 __device__ __forceinline__ AtTile at_find(const KvBatch &b, const KvAttn &a, const uint64_t *pre, uint64_t x)
 {
     int lo = 0, hi = b.n_seqs - 1;   // the last sequence that starts at or ahead of x
@@ -242,7 +292,7 @@ __device__ __forceinline__ AtTile at_find(const KvBatch &b, const KvAttn &a, con
     t.head = (int)(r / per);
     t.start = pre[lo] + per * t.head;
     for (t.t = 0;; t.t++) {
-        t.span = at_span<SLOG>(b, a, t.len, t.rows, t.t);
+        t.span = at_span<COLS, SLOG>(b, a, t.len, t.rows, t.t);
         if (x < t.start + AT_LEAD + t.span.n) return t;
         t.start += AT_LEAD + t.span.n;
     }
@@ -258,12 +308,13 @@ __global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBat
     typedef AtOps<E> Ops;
     constexpr int U = E::U, TK = U / 4, DS = D / (4 * U), DT = D / 16;
     constexpr int STEP = 4 * U, SLOG = U == 4 ? 4 : 5;
+    constexpr uint32_t EXP = U == 4 ? 0x7f800000u : Ops::PSHIFT != 0.0f ? 0x7c00u : 0x7f80u;   // all ones: not finite
     constexpr int LDO = D + 4;   // floats of a column in LDS: the four lanes of a column 16 bytes apart, columns over all banks
     extern __shared__ uint64_t pre[];
     __shared__ __align__(16) float so[AT_WAVES][AT_COLS][LDO];
     __shared__ float sm[AT_WAVES][AT_COLS], sl[AT_WAVES][AT_COLS];
     __shared__ uint64_t red[AT_WAVES];
-    at_prefix<SLOG, AT_THREADS>(b, a, pre, red);
+    at_prefix<AT_COLS, SLOG, AT_THREADS>(b, a, pre, red);
     float *const work = reinterpret_cast<float *>(joins + gridDim.x);
     const uint64_t W = pre[b.n_seqs];
     const uint32_t n = kv_parts(W, gridDim.x, AT_LEAST);
@@ -281,7 +332,7 @@ __global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBat
     const float qscale = (float)(a.scale * 1.4426950408889634);   // probabilities are powers of two
 
     for (uint64_t x = x0; x < x1;) {
-        const AtTile t = at_find<SLOG>(b, a, pre, x);
+        const AtTile t = at_find<AT_COLS, SLOG>(b, a, pre, x);
         const uint64_t own = t.start + AT_LEAD, tend = own + t.span.n;
         x = tend;
         if (own >= x1) break;    // the next workgroup's
@@ -350,14 +401,8 @@ __global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBat
                     uint32_t w[4] = {fv[d].x, fv[d].y, fv[d].z, fv[d].w};
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        if (U == 4) {
-                            w[i] &= keep[i];
-                            if (ROWS) odd |= (w[i] & 0x7f800000u) == 0x7f800000u;
-                        } else {
-                            w[i] &= (keep[(2 * i) % U] & 0xffffu) | (keep[(2 * i + 1) % U] & 0xffff0000u);
-                            constexpr uint32_t X = Ops::PSHIFT != 0.0f ? 0x7c00u : 0x7f80u;
-                            if (ROWS) odd |= (w[i] & X) == X || (w[i] & (X << 16)) == X << 16;
-                        }
+                        w[i] &= U == 4 ? keep[i % U] : (keep[(2 * i) % U] & 0xffffu) | (keep[(2 * i + 1) % U] & 0xffff0000u);
+                        if (ROWS) odd |= (w[i] & EXP) == EXP || (U == 8 && (w[i] & (EXP << 16)) == EXP << 16);
                     }
                     fv[d] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
@@ -380,32 +425,39 @@ __global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBat
                 p[e] = __builtin_amdgcn_exp2f(sc[e] - sub);
                 l += p[e];
             }
-            const typename Ops::P pp = Ops::split(p);
             if (ROWS && p0 != p1 && __any(odd)) {
-                // column by column, each over what it sees: 0 times such a value must not reach the others
-                for (int c = 0; c < ncol; c++) {
-                    const int cp = __builtin_amdgcn_readlane(pos, c), cl = __builtin_amdgcn_readlane(low, c);
-                    uint32_t keep[U];
+                // Such values leave the product, where 0 times one would reach
+                // the rows that do not see it, and are added one by one: lane
+                // L holds dimension L % 16 of unit L / 16, and its probability
+                // for this lane's column is in lane (column, unit).
 #pragma unroll
-                    for (int e = 0; e < U; e++)
-                        keep[e] = up + e <= cp && (up + e >= cl || up + e < sinks) ? 0xffffffffu : 0u;
+                for (int d = 0; d < DT; d++) {
+                    uint32_t w[4] = {fv[d].x, fv[d].y, fv[d].z, fv[d].w};
 #pragma unroll
-                    for (int d = 0; d < DT; d++) {
-                        uint32_t w[4] = {fv[d].x, fv[d].y, fv[d].z, fv[d].w};
+                    for (int e = 0; e < U; e++) {
+                        const int sh = U == 4 ? 0 : 16 * (e & 1);
+                        const uint32_t bits = U == 4 ? w[e % 4] : (w[e / 2] >> sh) & 0xffffu;
+                        const bool bad = (bits & EXP) == EXP;
+                        for (uint64_t who = __ballot(bad); who; who &= who - 1) {
+                            const int L = __builtin_ctzll(who);
+                            const float v = at_value(E{}, __builtin_amdgcn_readlane(bits, L));
+                            const float pr = __shfl(p[e], (L & 48) | col, WAVE);
+                            const int at = base + U * (L >> 4) + e;
+                            const bool sees = at <= pos && (at >= low || at < sinks);
+                            const float add = sees && (L & 15) >> 2 == j ? pr * v : 0.0f;
 #pragma unroll
-                        for (int i = 0; i < 4; i++)
-                            w[i] &= U == 4 ? keep[i % U]
-                                           : (keep[(2 * i) % U] & 0xffffu) | (keep[(2 * i + 1) % U] & 0xffff0000u);
-                        const f4_t add = Ops::mul(make_uint4(w[0], w[1], w[2], w[3]), pp, f4_t{0.0f, 0.0f, 0.0f, 0.0f});
-                        #pragma unroll
-                        for (int r = 0; r < 4; r++) o[d][r] += col == c ? add[r] : 0.0f;
+                            for (int r = 0; r < 4; r++) o[d][r] += (L & 3) == r ? add : 0.0f;
+                        }
+                        if (bad) w[U == 4 ? e % 4 : e / 2] &= U == 4 ? 0u : 0xffff0000u >> sh;
                     }
+                    fv[d] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
-            } else {
-#pragma unroll
-                for (int d = 0; d < DT; d++) o[d] = Ops::mul(fv[d], pp, o[d]);
             }
+            const typename Ops::P pp = Ops::split(p);
+#pragma unroll
+            for (int d = 0; d < DT; d++) o[d] = Ops::mul(fv[d], pp, o[d]);
         };
+
         // ---- the first loads, then q in planes ----
         int i = i0 + wave;
         int gk, gv, now, gk1, gv1;
@@ -493,7 +545,7 @@ __global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBat
         __syncthreads();
         // whole: the result; else this workgroup's slot for a tile that began before it, or that goes on behind it
         const bool mine = i0 == 0 && i1 == t.span.n;
-        float *slot = work + (size_t)(2 * blockIdx.x + (i0 == 0 ? 1 : 0)) * attn_slot(D);
+        float *slot = work + (size_t)(2 * blockIdx.x + (i0 == 0 ? 1 : 0)) * attn_slot(AT_COLS, D);
         for (int e = tid; e < ncol * (D / 4); e += AT_THREADS) {
             const int c = e / (D / 4), d = e % (D / 4) * 4;
             float M = sm[0][c];
@@ -533,20 +585,309 @@ __global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBat
     if (tid == 0) joins[blockIdx.x] = AtJoin{left_count, left_row0, left_c0, left_ncol, left_head, {0, 0, 0}};
 }
 
-// The tiles that cuts separate: workgroup (w, c) takes column c of the tile
-// that part w leaves to those behind it.  A thread holds four dimensions, and
-// 256 / (D / 4) classes of parts their running maximum and sums.
-template <int D>
+// ---- many rows ----------------------------------------------------------------------
+
+// The same over tiles of 128 columns, 32 a wave, for calls whose columns are
+// many: keys and values go through LDS, where the four waves read them, and
+// 32x32 instructions.  A stage is P positions of K, [D / U][P] units, and of
+// V, [P / U][D] units, copied straight from the pool (asynchronously, 16 bytes
+// a lane) while the stage before it is worked on; K's positions are stored in
+// the order of the instruction's rows, so that every read of LDS is of
+// consecutive units.  Row m = 8 a + 4 h + b of 32 is position 16 (a / 2) + 8 h
+// + 4 (a % 2) + b of 16-bit types, m of fp32: the scores of a lane's half h
+// then are those of whole units of V.
+template <class E, int D>
+__global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvBatch b, KvAttn a,
+                                                                            AtJoin *__restrict__ joins)
+{
+    typedef AtOps<E> Ops;
+    constexpr int U = E::U, P = U == 4 ? 32 : 64, SLOG = U == 4 ? 5 : 6;
+    constexpr int KU = D / U * P, VU = P / U * D;          // units of a stage
+    constexpr int NK = KU / AT_THREADS, NV = VU / AT_THREADS;
+    constexpr int DS = D / (2 * U), DT = D / 32, HALVES = P / 32, NI = 16 / U;
+    constexpr uint32_t EXP = U == 4 ? 0x7f800000u : Ops::PSHIFT != 0.0f ? 0x7c00u : 0x7f80u;
+    static_assert(KU % AT_THREADS == 0 && VU % AT_THREADS == 0, "copies by whole workgroups");
+    extern __shared__ uint64_t pre[];
+    __shared__ __align__(16) uint4 sk[2][KU], sv[2][VU];
+    __shared__ uint64_t red[AT_WAVES];
+    at_prefix<AW_COLS, SLOG, AT_THREADS>(b, a, pre, red);
+    float *const work = reinterpret_cast<float *>(joins + gridDim.x);
+    const uint64_t W = pre[b.n_seqs];
+    const uint32_t n = kv_parts(W, gridDim.x, AT_LEAST);
+    // parts in a row on one XCD (workgroups go to the eight in turn): they read the same keys and values
+    const uint32_t per = (gridDim.x + 7) / 8;
+    const uint32_t part = gridDim.x % 8 ? blockIdx.x : blockIdx.x % 8 * per + blockIdx.x / 8;
+    const uint64_t x0 = W && part < n ? kv_cut(W, n, part) : 0;
+    const uint64_t x1 = W && part < n ? kv_cut(W, n, part + 1) : 0;
+    int left_count = 0, left_row0 = 0, left_c0 = 0, left_ncol = 0, left_head = 0;   // this workgroup's AtJoin
+
+    const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
+    const int col = lane & 31, h = lane >> 5;
+    const int nkv = b.s.n_kv_heads, ps = b.s.page_size, nh = a.n_heads, grp = a.group;
+    const size_t vbase = (size_t)nkv * ps * D * (16 / U);
+    const float qscale = (float)(a.scale * 1.4426950408889634);
+    // the position that this lane copies of K (unit tid of AT_THREADS: position tid % P in the rows' order)
+    const int kr = tid % P % 32;
+    const int kp = tid % P / 32 * 32 + (U == 4 ? kr : 16 * (kr >> 4) + 8 * (kr >> 2 & 1) + 4 * (kr >> 3 & 1) + (kr & 3));
+    const uint32_t lk = lds_u32(&sk[0][wave * WAVE]), lv = lds_u32(&sv[0][wave * WAVE]);
+
+    for (uint64_t x = x0; x < x1;) {
+        const AtTile t = at_find<AW_COLS, SLOG>(b, a, pre, x);
+        const uint64_t own = t.start + AT_LEAD, tend = own + t.span.n;
+        x = tend;
+        if (own >= x1) break;    // the next workgroup's
+        const int i0 = x0 > own ? (int)(x0 - own) : 0;
+        const int i1 = (int)((tend < x1 ? tend : x1) - own);
+        const int c0 = t.t * AW_COLS, ncol = min(AW_COLS, t.rows * grp - c0);
+        // this wave's columns, those behind the tile's last doing what that one does
+        const bool any = wave * 32 < ncol;
+        const int w0 = min(wave * 32, ncol - 1), w1 = min(wave * 32 + 31, ncol - 1);
+        const int cc = c0 + min(wave * 32 + col, ncol - 1), cr = cc / grp;
+        const int p0 = t.len - t.rows + (c0 + w0) / grp, p1 = t.len - t.rows + (c0 + w1) / grp;
+        const int pos = t.len - t.rows + cr;
+        const int low = a.window && pos >= 0 ? max(pos - a.window + 1, 0) : 0;
+        const int low0 = a.window && p0 >= 0 ? max(p0 - a.window + 1, 0) : 0;
+        const int low1 = a.window && p1 >= 0 ? max(p1 - a.window + 1, 0) : 0;
+        const int sinks = a.sinks;
+
+        int ek, ev[NV];     // table entries of the next copies
+        auto entries = [&](int i) {
+            const int base = kv_base(t.span, min(i, i1 - 1), SLOG);
+            ek = kv_entry(b, t.seq, base + kp);
+#pragma unroll
+            for (int k = 0; k < NV; k++) ev[k] = kv_entry(b, t.seq, base + (k * AT_THREADS + tid) / D * U);
+        };
+        // (returns which of the stage's positions, in the rows' order, have a page)
+        auto copy = [&](int i, int buf) -> uint64_t {
+            const int base = kv_base(t.span, i, SLOG);
+            const int at = base + kp, kg = kv_page_of(b, at, ek);
+            const char *src = b.pool + (size_t)max(kg, 0) * b.s.page_bytes +
+                              ((size_t)(t.head * (D / U) + tid / P) * ps + (at & (ps - 1))) * 16;
+#pragma unroll
+            for (int k = 0; k < NK; k++)
+                dma16(src + (size_t)k * (AT_THREADS / P) * ps * 16, lk + (buf * KU + k * AT_THREADS) * 16);
+#pragma unroll
+            for (int k = 0; k < NV; k++) {
+                const int g = k * AT_THREADS + tid, v = base + g / D * U;
+                dma16(b.pool + (size_t)max(kv_page_of(b, v, ev[k]), 0) * b.s.page_bytes + vbase +
+                          ((size_t)(t.head * (ps / U) + (v & (ps - 1)) / U) * D + g % D) * 16,
+                      lv + (buf * VU + k * AT_THREADS) * 16);
+            }
+            return __ballot(kg >= 0);
+        };
+        entries(i0);
+        lds_barrier();       // the stages are free: every wave is done with the tile before
+        uint64_t pages = copy(i0, 0), pages_next = 0;
+        entries(i0 + 1);
+
+        // ---- q in planes ----
+        typename Ops::Q q[DS];
+        float unscale = 1.0f;
+        {
+            f4_t v[DS][U / 4];
+            const float *src = a.q + ((size_t)(t.row0 + cr) * nh + t.head * grp + cc % grp) * D + h * U;
+#pragma unroll
+            for (int s = 0; s < DS; s++)
+#pragma unroll
+                for (int e = 0; e < U / 4; e++) v[s][e] = *reinterpret_cast<const f4u_t *>(src + 2 * U * s + 4 * e);
+            float up = 1.0f;
+            if (Ops::PSHIFT != 0.0f) {
+                // the largest to [2^14, 2^15)
+                float big = 0.0f;
+#pragma unroll
+                for (int s = 0; s < DS; s++)
+#pragma unroll
+                    for (int e = 0; e < U; e++) big = fmaxf(big, fabsf(v[s][e / 4][e % 4] * qscale));
+                const int f = min(268 - (int)(__float_as_uint(half_max(big)) >> 23), 253);
+                unscale = __uint_as_float((uint32_t)(254 - f) << 23);
+                up = __uint_as_float((uint32_t)f << 23);
+            }
+#pragma unroll
+            for (int s = 0; s < DS; s++) {
+                float xs[U];
+#pragma unroll
+                for (int e = 0; e < U; e++) xs[e] = v[s][e / 4][e % 4] * qscale * up;
+                q[s] = Ops::split(xs);
+            }
+        }
+
+        float m = -INFINITY, l = 0.0f;
+        f16_t o[DT];
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[d] = f16_t{};
+
+        // 32 positions from `base` on: half hf of the stage in `buf`
+        auto work_half = [&](int base, int buf, int hf, uint32_t got, auto masked) {
+            constexpr bool MASK = decltype(masked)::value;
+            f16_t sc = {};
+#pragma unroll
+            for (int s = 0; s < DS; s++) sc = Ops::mul(sk[buf][(2 * s + h) * P + 32 * hf + col], q[s], sc);
+            // register r: position at(r) of these
+            auto at = [&](int r) { return U == 4 ? 8 * (r >> 2) + 4 * h + (r & 3) : 16 * (r >> 3) + 8 * h + (r & 7); };
+            bool page[NI];
+#pragma unroll
+            for (int r = 0; r < 16; r++) sc[r] *= unscale;
+            if (MASK) {
+#pragma unroll
+                for (int i = 0; i < NI; i++) page[i] = got >> (8 * (i * U >> 2) + 4 * h) & 1;   // a unit has one page
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int p = base + at(r);
+                    if (!(page[r / U] && p <= pos && (p >= low || p < sinks))) sc[r] = -INFINITY;
+                }
+            }
+            float mx = sc[0];
+#pragma unroll
+            for (int r = 1; r < 16; r++) mx = fmaxf(mx, sc[r]);
+            mx = fmaxf(m, half_max(mx));
+            if (__any(mx > m)) {
+                const float f = __builtin_amdgcn_exp2f(m - (mx == -INFINITY ? 0.0f : mx));
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[d] *= f;
+                m = mx;
+            }
+            const float sub = (m == -INFINITY ? 0.0f : m) - Ops::PSHIFT;
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                sc[r] = __builtin_amdgcn_exp2f(sc[r] - sub);
+                l += sc[r];
+            }
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                float ps_[U];
+#pragma unroll
+                for (int e = 0; e < U; e++) ps_[e] = sc[i * U + e];
+                const typename Ops::P pp = Ops::split(ps_);
+                const int unit = 32 / U * hf + 2 * i + h;
+                uint32_t keep[4];
+                if (MASK) {
+                    // what none of this wave's rows sees may hold anything
+                    uint32_t k1[U];
+#pragma unroll
+                    for (int e = 0; e < U; e++) {
+                        const int p = base + at(i * U + e);
+                        k1[e] = page[i] && p <= p1 && (p >= low0 || p < sinks) ? 0xffffffffu : 0u;
+                    }
+#pragma unroll
+                    for (int w = 0; w < 4; w++)
+                        keep[w] = U == 4 ? k1[w % U] : (k1[(2 * w) % U] & 0xffffu) | (k1[(2 * w + 1) % U] & 0xffff0000u);
+                }
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    uint4 v = sv[buf][unit * D + 32 * d + col];
+                    if (MASK) {
+                        uint32_t w[4] = {v.x & keep[0], v.y & keep[1], v.z & keep[2], v.w & keep[3]};
+                        bool odd = false;
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            odd |= (w[k] & EXP) == EXP || (U == 8 && (w[k] & (EXP << 16)) == EXP << 16);
+                        if (p0 != p1 && __any(odd)) {
+                            // values that are not finite, one by one, as in the narrow form
+#pragma unroll
+                            for (int e = 0; e < U; e++) {
+                                const int sh = U == 4 ? 0 : 16 * (e & 1);
+                                const uint32_t bits = U == 4 ? w[e % 4] : (w[e / 2] >> sh) & 0xffffu;
+                                const bool bad = (bits & EXP) == EXP;
+                                for (uint64_t who = __ballot(bad); who; who &= who - 1) {
+                                    const int L = __builtin_ctzll(who);
+                                    const float val = at_value(E{}, __builtin_amdgcn_readlane(bits, L));
+                                    const float pr = __shfl(ps_[e], (L & 32) | col, WAVE);
+                                    const int p = base + (U == 4 ? 8 * i + 4 * (L >> 5) : 16 * i + 8 * (L >> 5)) + e;
+                                    const bool sees = p <= pos && (p >= low || p < sinks);
+                                    // dimension L % 32 is register 4 (dim / 8) + dim % 4 of half dim / 4 % 2
+                                    const float add = sees && (L >> 2 & 1) == h ? pr * val : 0.0f;
+#pragma unroll
+                                    for (int r = 0; r < 16; r++)
+                                        o[d][r] += ((L >> 3 & 3) * 4 + (L & 3)) == r ? add : 0.0f;
+                                }
+                                if (bad) w[U == 4 ? e % 4 : e / 2] &= U == 4 ? 0u : 0xffff0000u >> sh;
+                            }
+                        }
+                        v = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    o[d] = Ops::mul(v, pp, o[d]);
+                }
+            }
+        };
+        for (int i = i0; i < i1; i++) {
+            const int buf = (i - i0) & 1;
+            wait_vm<0>();
+            lds_barrier();       // this stage is there, and the other one free
+            if (i + 1 < i1) {
+                pages_next = copy(i + 1, buf ^ 1);
+                entries(i + 2);
+            }
+            const int base = kv_base(t.span, i, SLOG);
+#pragma unroll 1
+            for (int hf = 0; hf < HALVES; hf++) {
+                const int hb = base + 32 * hf;
+                if (!any || hb > p1 || (hb + 32 <= low0 && hb >= sinks)) continue;   // nobody's
+                const uint32_t got = (uint32_t)(pages >> 32 * hf);
+                const bool whole = hb + 31 <= p0 && (hb >= low1 || hb + 32 <= sinks) && got == 0xffffffffu;
+                if (whole) work_half(hb, buf, hf, got, std::false_type{});
+                else work_half(hb, buf, hf, got, std::true_type{});
+            }
+            pages = pages_next;
+        }
+
+        // ---- results, or this workgroup's slot ----
+        l = half_sum(l);
+        const bool mine = i0 == 0 && i1 == t.span.n;
+        if (wave * 32 + col < ncol) {
+            const int c = wave * 32 + col;
+            if (mine) {
+                float *dst = a.out + ((size_t)(t.row0 + cr) * nh + t.head * grp + cc % grp) * D;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const f4_t s = {o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
+                        *reinterpret_cast<f4u_t *>(dst + 32 * d + 8 * k + 4 * h) = l == 0.0f ? s : s / l;
+                    }
+            } else {
+                float *slot = work + (size_t)(2 * part + (i0 == 0 ? 1 : 0)) * attn_slot(AW_COLS, D);
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        *reinterpret_cast<f4_t *>(slot + c * D + 32 * d + 8 * k + 4 * h) =
+                            f4_t{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
+                if (h == 0) {
+                    slot[AW_COLS * D + c] = m;
+                    slot[AW_COLS * (D + 1) + c] = l;
+                }
+            }
+        }
+        if (i0 == 0 && !mine) {
+            left_count = (int)(kv_part(W, n, tend - 1) - part) + 1;
+            left_row0 = t.row0;
+            left_c0 = c0;
+            left_ncol = ncol;
+            left_head = t.head;
+        }
+    }
+    if (tid == 0) joins[part] = AtJoin{left_count, left_row0, left_c0, left_ncol, left_head, {0, 0, 0}};
+}
+
+// The tiles that cuts separate: workgroup (w, y) takes columns y JC .. of the
+// tile that part w leaves to those behind it.  A thread holds four dimensions
+// of a column, and CL classes of parts their running maximum and sums.
+template <int COLS, int D, int JC>
 __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttn a, const AtJoin *__restrict__ joins)
 {
-    constexpr int LN = D / 4, CL = 256 / LN, AHEAD = 8;
-    __shared__ float sm[CL], sl[CL];
-    __shared__ __align__(16) f4_t so[CL][LN];
+    constexpr int LN = D / 4, CL = 256 / (LN * JC), AHEAD = 8;
+    __shared__ float sms[JC][CL], sls[JC][CL];
+    __shared__ __align__(16) f4_t sos[JC][CL][LN];
     const AtJoin t = joins[blockIdx.x];
-    const int c = blockIdx.y;
-    if (c >= t.ncol || t.count == 0) return;
+    if ((int)blockIdx.y * JC >= t.ncol || t.count == 0) return;
     const float *work = reinterpret_cast<const float *>(joins + gridDim.x);
-    const int cl = threadIdx.x / LN, ln = threadIdx.x % LN;
+    // (threads behind the last column or class do its work beside it and store nothing)
+    const int jc = threadIdx.x / (LN * CL) % JC, ln = threadIdx.x % LN;
+    const int cl = threadIdx.x < LN * CL * JC ? threadIdx.x / LN % CL : CL;
+    const int c = min((int)blockIdx.y * JC + jc, t.ncol - 1);
+    float *const sm = sms[jc], *const sl = sls[jc];
+    f4_t(*const so)[LN] = sos[jc];
     float M = -INFINITY, L = 0.0f;
     f4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
     if (cl < CL)
@@ -556,9 +897,9 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttn a, const AtJoi
 #pragma unroll
             for (int u = 0; u < AHEAD; u++) {
                 const int k = min(k0 + u * CL, t.count - 1);
-                const float *s = work + (size_t)(2 * (blockIdx.x + k) + (k == 0)) * attn_slot(D);
-                m[u] = s[AT_COLS * D + c];
-                l[u] = s[AT_COLS * (D + 1) + c];
+                const float *s = work + (size_t)(2 * (blockIdx.x + k) + (k == 0)) * attn_slot(COLS, D);
+                m[u] = s[COLS * D + c];
+                l[u] = s[COLS * (D + 1) + c];
                 o[u] = *reinterpret_cast<const f4_t *>(s + c * D + 4 * ln);
             }
             float top = M;
@@ -586,7 +927,7 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttn a, const AtJoi
         }
     }
     __syncthreads();
-    if (threadIdx.x >= LN) return;
+    if (cl != 0 || (int)blockIdx.y * JC + jc >= t.ncol) return;
     const int top = min(CL, t.count);
     M = sm[0];
     for (int k = 1; k < top; k++) M = fmaxf(M, sm[k]);
@@ -606,17 +947,25 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttn a, const AtJoi
 template <class E, int D>
 static void attn_launch_d(qq_ctx *ctx, const qq_kv *kv, const KvBatch &b, const KvAttn &a)
 {
-    const int parts = attn_parts(ctx, D);
     const size_t shm = (size_t)(b.n_seqs + 1) * sizeof(uint64_t);
     AtJoin *joins = reinterpret_cast<AtJoin *>(kv->work);
+    // Many rows a sequence: more than two narrow tiles' columns.
+    const bool wide = b.row_start && (int64_t)b.n_rows * a.group > (int64_t)2 * AT_COLS * b.n_seqs;
+    const int parts = wide ? wide_parts(ctx) : attn_parts(ctx, D);
     prof_begin(ctx, K_KV_ATTN);
-    if (b.row_start)
+    if (wide)
+        QQ_LAUNCH(ctx, (kv_attn_wide_kernel<E, D>), dim3(parts), dim3(AT_THREADS), shm, b, a, joins);
+    else if (b.row_start)
         QQ_LAUNCH(ctx, (kv_attn_kernel<E, D, true>), dim3(parts), dim3(AT_THREADS), shm, b, a, joins);
     else
         QQ_LAUNCH(ctx, (kv_attn_kernel<E, D, false>), dim3(parts), dim3(AT_THREADS), shm, b, a, joins);
     prof_begin(ctx, K_KV_JOIN);
-    const int cols = std::min(AT_COLS, b.row_start ? AT_COLS : a.group);
-    QQ_LAUNCH(ctx, kv_attn_join_kernel<D>, dim3(parts, cols), dim3(256), 0, a, joins);
+    constexpr int JC = 128 / (D / 4);   // two classes of parts: a wide tile's are few
+    if (wide)
+        QQ_LAUNCH(ctx, (kv_attn_join_kernel<AW_COLS, D, JC>), dim3(parts, (AW_COLS + JC - 1) / JC), dim3(256), 0, a, joins);
+    else
+        QQ_LAUNCH(ctx, (kv_attn_join_kernel<AT_COLS, D, 1>),
+                  dim3(parts, b.row_start ? AT_COLS : std::min(AT_COLS, a.group)), dim3(256), 0, a, joins);
     prof_end(ctx);
 }
 
