@@ -156,10 +156,9 @@ struct AtOps<KvF16> {
     {
         Q q;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            q.h[i] = (_Float16)x[i];
-            q.l[i] = (_Float16)(x[i] - (float)q.h[i]);
-        }
+        for (int i = 0; i < 8; i++) q.h[i] = (_Float16)x[i];
+#pragma unroll
+        for (int i = 0; i < 8; i++) q.l[i] = (_Float16)fmaf(-1.0f, (float)q.h[i], x[i]);
         return q;
     }
     static __device__ __forceinline__ f4_t mul(const uint4 &a, const Q &q, f4_t c)
@@ -228,6 +227,9 @@ __device__ __forceinline__ float half_sum(float v)
 
 // ---- the plan, in every workgroup ---------------------------------------------------
 
+// Tiles count by sequence, then column tile, the same for every key/value
+// head; heads are the outer order.  A thread weighs T / NT tiles in a row; a
+// step is found by a search over those runs and a walk through one of them.
 struct AtTile {
     int seq, head, t;        // sequence, key/value head, column tile
     int row0, rows, len;     // the sequence's new rows and length
@@ -235,68 +237,168 @@ struct AtTile {
     KvSpan span;
 };
 
-template <int COLS, int SLOG>
-__device__ __forceinline__ KvSpan at_span(const KvBatch &b, const KvAttn &a, int len, int rows, int t)
+template <int NT>
+struct AtPlan {
+    uint64_t runs[NT + 1];   // steps of one head ahead of every thread's run
+    uint64_t red[NT / WAVE];
+};
+// ... and in dynamic LDS, per sequence: its length, and where a sequence may
+// have other than one row, its tiles' number among all, its first row, its rows
+static size_t at_plan_bytes(const KvBatch &b) { return (size_t)(b.row_start ? 4 * b.n_seqs + 1 : b.n_seqs) * sizeof(int); }
+
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint64_t uni64(uint64_t v)
 {
-    return kv_tile_span(len, rows, t, COLS, a.group, b.stride << b.s.page_log, a.window, a.sinks, SLOG);
+    return (uint64_t)(uint32_t)uni((int)(v >> 32)) << 32 | (uint32_t)uni((int)v);
 }
 
-// pre[i] = steps of the sequences ahead of i, for i <= n_seqs (threads: the whole workgroup).
-template <int COLS, int SLOG, int NT>
-__device__ __forceinline__ void at_prefix(const KvBatch &b, const KvAttn &a, uint64_t *pre, uint64_t *red)
+// Exclusive prefix of one value a thread over the workgroup, and the total.
+template <class V, int NT>
+__device__ __forceinline__ V at_scan(V v, V &total, uint64_t *red)
 {
-    const int per = (b.n_seqs + NT - 1) / NT, tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
-    const int s0 = min(tid * per, b.n_seqs), s1 = min(s0 + per, b.n_seqs);
-    uint64_t sum = 0;
-    for (int s = s0; s < s1; s++) {
-        int r0, r1;
-        kv_rows(b, s, r0, r1);
-        const int len = max(b.len[s], 0), n = kv_tiles(r1 - r0, a.group, COLS);
-        uint64_t steps = 0;
-        for (int t = 0; t < n; t++) steps += at_span<COLS, SLOG>(b, a, len, r1 - r0, t).n + AT_LEAD;
-        pre[s] = sum;      // within this thread's run
-        sum += steps * b.s.n_kv_heads;
-    }
-    uint64_t inc = sum;
+    const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
+    V inc = v;
 #pragma unroll
     for (int o = 1; o < WAVE; o <<= 1) {
-        const uint64_t up = __shfl_up(inc, o, WAVE);
+        const V up = __shfl_up(inc, o, WAVE);
         if (lane >= o) inc += up;
     }
+    __syncthreads();
     if (lane == WAVE - 1) red[wave] = inc;
     __syncthreads();
-    uint64_t off = inc - sum;
-    for (int w = 0; w < wave; w++) off += red[w];
-    for (int s = s0; s < s1; s++) pre[s] += off;
-    if (tid == NT - 1) pre[b.n_seqs] = off + sum;
-    __syncthreads();
+    V off = inc - v;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < NT / WAVE; w++) {
+        if (w < wave) off += (V)red[w];
+        total += (V)red[w];
+    }
+    return off;
 }
 
-// The tile that holds step x.
-template <int COLS, int SLOG>
-__device__ __forceinline__ AtTile at_find(const KvBatch &b, const KvAttn &a, const uint64_t *pre, uint64_t x)
-{
-    int lo = 0, hi = b.n_seqs - 1;   // the last sequence that starts at or ahead of x
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (pre[mid] <= x) lo = mid;
-        else hi = mid - 1;
+template <bool ROWS, int COLS, int SLOG, int NT>
+struct AtWork {
+    const KvBatch &b;
+    const KvAttn &a;
+    AtPlan<NT> &p;
+    int *const len, *const first, *const row0, *const rows;
+    int per;          // tiles of a run
+    int each;         // tiles of a sequence of one row
+    uint64_t S;       // steps of one head
+
+    __device__ AtWork(const KvBatch &b_, const KvAttn &a_, AtPlan<NT> &p_, int *lds)
+        : b(b_), a(a_), p(p_), len(lds), first(lds + b_.n_seqs), row0(lds + 2 * b_.n_seqs + 1),
+          rows(lds + 3 * b_.n_seqs + 1)
+    {
+        each = kv_tiles(1, a.group, COLS);
     }
-    AtTile t;
-    t.seq = lo;
-    int r1;
-    kv_rows(b, lo, t.row0, r1);
-    t.rows = r1 - t.row0;
-    t.len = max(b.len[lo], 0);
-    const uint64_t per = (pre[lo + 1] - pre[lo]) / b.s.n_kv_heads, r = x - pre[lo];
-    t.head = (int)(r / per);
-    t.start = pre[lo] + per * t.head;
-    for (t.t = 0;; t.t++) {
-        t.span = at_span<COLS, SLOG>(b, a, t.len, t.rows, t.t);
-        if (x < t.start + AT_LEAD + t.span.n) return t;
-        t.start += AT_LEAD + t.span.n;
+    __device__ __forceinline__ KvSpan span(int ln, int rw, int t) const
+    {
+        return kv_tile_span(ln, rw, t, COLS, a.group, b.stride << b.s.page_log, a.window, a.sinks, SLOG);
     }
-}
+    // The sequence of tile g and its tile there.
+    __device__ __forceinline__ void place(int g, int &seq, int &t) const
+    {
+        if (!ROWS) {
+            seq = each == 1 ? g : g / each;
+            t = each == 1 ? 0 : g - seq * each;
+            return;
+        }
+        int lo = 0, hi = b.n_seqs - 1;   // the last sequence that starts at or ahead of g
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (first[mid] <= g) lo = mid;
+            else hi = mid - 1;
+        }
+        seq = lo;
+        t = g - first[lo];
+    }
+    __device__ __forceinline__ void next(int &seq, int &t) const
+    {
+        t++;
+        if (!ROWS) {
+            if (t == each) {
+                t = 0;
+                seq++;
+            }
+            return;
+        }
+        if (t < first[seq + 1] - first[seq]) return;
+        t = 0;
+        do seq++;
+        while (seq < b.n_seqs && first[seq + 1] == first[seq]);
+    }
+    // All steps of the call (the whole workgroup).
+    __device__ __forceinline__ uint64_t plan()
+    {
+        const int tid = threadIdx.x;
+        int T = b.n_seqs * each;
+        for (int s = tid; s < b.n_seqs; s += NT) len[s] = max(b.len[s], 0);
+        if (ROWS) {
+            const int run = (b.n_seqs + NT - 1) / NT, s0 = min(tid * run, b.n_seqs), s1 = min(s0 + run, b.n_seqs);
+            int sum = 0;
+            for (int s = s0; s < s1; s++) {
+                int r0, r1;
+                kv_rows(b, s, r0, r1);
+                row0[s] = r0;
+                rows[s] = r1 - r0;
+                first[s] = sum;
+                sum += kv_tiles(r1 - r0, a.group, COLS);
+            }
+            const int off = at_scan<int, NT>(sum, T, p.red);
+            for (int s = s0; s < s1; s++) first[s] += off;
+            if (tid == 0) first[b.n_seqs] = T;
+        }
+        __syncthreads();
+        T = uni(T);
+        per = (T + NT - 1) / NT;
+        const int g0 = min(tid * per, T), g1 = min(g0 + per, T);
+        uint64_t sum = 0;
+        if (g0 < g1) {
+            int seq, t;
+            place(g0, seq, t);
+            for (int g = g0;;) {
+                sum += span(len[seq], ROWS ? rows[seq] : 1, t).n + AT_LEAD;
+                if (++g == g1) break;
+                next(seq, t);
+            }
+        }
+        const uint64_t off = at_scan<uint64_t, NT>(sum, S, p.red);
+        p.runs[tid] = off;
+        if (tid == 0) p.runs[NT] = S;
+        __syncthreads();
+        S = uni64(S);
+        return S * b.s.n_kv_heads;
+    }
+    // The tile that holds step x.
+    __device__ __forceinline__ AtTile find(uint64_t x) const
+    {
+        AtTile t;
+        t.head = (int)(x / S);
+        const uint64_t base = S * t.head, r = x - base;
+        int lo = 0, hi = NT - 1;         // the last run that starts at or ahead of r
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (uni64(p.runs[mid]) <= r) lo = mid;
+            else hi = mid - 1;
+        }
+        uint64_t start = uni64(p.runs[lo]);
+        place(lo * per, t.seq, t.t);
+        for (;;) {
+            t.seq = uni(t.seq);
+            t.t = uni(t.t);
+            t.len = uni(len[t.seq]);
+            t.rows = ROWS ? uni(rows[t.seq]) : 1;
+            t.span = span(t.len, t.rows, t.t);
+            if (r < start + AT_LEAD + t.span.n) break;
+            start += AT_LEAD + t.span.n;
+            next(t.seq, t.t);
+        }
+        t.row0 = ROWS ? uni(row0[t.seq]) : t.seq;
+        t.start = base + start;
+        return t;
+    }
+};
 
 // ---- the kernel ---------------------------------------------------------------------
 
@@ -310,20 +412,20 @@ __global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBat
     constexpr int STEP = 4 * U, SLOG = U == 4 ? 4 : 5;
     constexpr uint32_t EXP = U == 4 ? 0x7f800000u : Ops::PSHIFT != 0.0f ? 0x7c00u : 0x7f80u;   // all ones: not finite
     constexpr int LDO = D + 4;   // floats of a column in LDS: the four lanes of a column 16 bytes apart, columns over all banks
-    extern __shared__ uint64_t pre[];
+    extern __shared__ int seqs[];
     __shared__ __align__(16) float so[AT_WAVES][AT_COLS][LDO];
     __shared__ float sm[AT_WAVES][AT_COLS], sl[AT_WAVES][AT_COLS];
-    __shared__ uint64_t red[AT_WAVES];
-    at_prefix<AT_COLS, SLOG, AT_THREADS>(b, a, pre, red);
+    __shared__ AtPlan<AT_THREADS> plan;
+    AtWork<ROWS, AT_COLS, SLOG, AT_THREADS> wk(b, a, plan, seqs);
     float *const work = reinterpret_cast<float *>(joins + gridDim.x);
-    const uint64_t W = pre[b.n_seqs];
+    const uint64_t W = wk.plan();
     const uint32_t n = kv_parts(W, gridDim.x, AT_LEAST);
     // (no steps, or fewer parts than workgroups: none for this one)
     const uint64_t x0 = W && blockIdx.x < n ? kv_cut(W, n, blockIdx.x) : 0;
     const uint64_t x1 = W && blockIdx.x < n ? kv_cut(W, n, blockIdx.x + 1) : 0;
     int left_count = 0, left_row0 = 0, left_c0 = 0, left_ncol = 0, left_head = 0;   // this workgroup's AtJoin
 
-    const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
+    const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = uni(tid / WAVE);
     const int col = lane & 15, j = lane >> 4;
     const int nkv = b.s.n_kv_heads, ps = b.s.page_size, nh = a.n_heads, grp = a.group;
     // K's operand row `col` is a position of unit ku; its unit of dimensions is j + 4 s
@@ -332,7 +434,7 @@ __global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBat
     const float qscale = (float)(a.scale * 1.4426950408889634);   // probabilities are powers of two
 
     for (uint64_t x = x0; x < x1;) {
-        const AtTile t = at_find<AT_COLS, SLOG>(b, a, pre, x);
+        const AtTile t = wk.find(x);
         const uint64_t own = t.start + AT_LEAD, tend = own + t.span.n;
         x = tend;
         if (own >= x1) break;    // the next workgroup's
@@ -392,9 +494,9 @@ __global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBat
                 for (int e = 0; e < U; e++) {
                     const int p = up + e;
                     const bool page = g >= 0;
-                    if (!(page && p <= pos && (p >= low || p < sinks))) sc[e] = -INFINITY;
+                    sc[e] = page & (p <= pos) & ((p >= low) | (p < sinks)) ? sc[e] : -INFINITY;
                     // what no row of the tile sees may hold anything
-                    keep[e] = page && p <= p1 && (p >= low0 || p < sinks) ? 0xffffffffu : 0u;
+                    keep[e] = page & (p <= p1) & ((p >= low0) | (p < sinks)) ? 0xffffffffu : 0u;
                 }
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
@@ -607,12 +709,12 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
     constexpr int DS = D / (2 * U), DT = D / 32, HALVES = P / 32, NI = 16 / U;
     constexpr uint32_t EXP = U == 4 ? 0x7f800000u : Ops::PSHIFT != 0.0f ? 0x7c00u : 0x7f80u;
     static_assert(KU % AT_THREADS == 0 && VU % AT_THREADS == 0, "copies by whole workgroups");
-    extern __shared__ uint64_t pre[];
+    extern __shared__ int seqs[];
     __shared__ __align__(16) uint4 sk[2][KU], sv[2][VU];
-    __shared__ uint64_t red[AT_WAVES];
-    at_prefix<AW_COLS, SLOG, AT_THREADS>(b, a, pre, red);
+    __shared__ AtPlan<AT_THREADS> plan;
+    AtWork<true, AW_COLS, SLOG, AT_THREADS> wk(b, a, plan, seqs);
     float *const work = reinterpret_cast<float *>(joins + gridDim.x);
-    const uint64_t W = pre[b.n_seqs];
+    const uint64_t W = wk.plan();
     const uint32_t n = kv_parts(W, gridDim.x, AT_LEAST);
     // parts in a row on one XCD (workgroups go to the eight in turn): they read the same keys and values
     const uint32_t per = (gridDim.x + 7) / 8;
@@ -621,7 +723,7 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
     const uint64_t x1 = W && part < n ? kv_cut(W, n, part + 1) : 0;
     int left_count = 0, left_row0 = 0, left_c0 = 0, left_ncol = 0, left_head = 0;   // this workgroup's AtJoin
 
-    const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
+    const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = uni(tid / WAVE);
     const int col = lane & 31, h = lane >> 5;
     const int nkv = b.s.n_kv_heads, ps = b.s.page_size, nh = a.n_heads, grp = a.group;
     const size_t vbase = (size_t)nkv * ps * D * (16 / U);
@@ -629,10 +731,12 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
     // the position that this lane copies of K (unit tid of AT_THREADS: position tid % P in the rows' order)
     const int kr = tid % P % 32;
     const int kp = tid % P / 32 * 32 + (U == 4 ? kr : 16 * (kr >> 4) + 8 * (kr >> 2 & 1) + 4 * (kr >> 3 & 1) + (kr & 3));
+    // the position of register r among 32
+    auto at = [&](int r) { return U == 4 ? 8 * (r >> 2) + 4 * h + (r & 3) : 16 * (r >> 3) + 8 * h + (r & 7); };
     const uint32_t lk = lds_u32(&sk[0][wave * WAVE]), lv = lds_u32(&sv[0][wave * WAVE]);
 
     for (uint64_t x = x0; x < x1;) {
-        const AtTile t = at_find<AW_COLS, SLOG>(b, a, pre, x);
+        const AtTile t = wk.find(x);
         const uint64_t own = t.start + AT_LEAD, tend = own + t.span.n;
         x = tend;
         if (own >= x1) break;    // the next workgroup's
@@ -649,6 +753,9 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
         const int low0 = a.window && p0 >= 0 ? max(p0 - a.window + 1, 0) : 0;
         const int low1 = a.window && p1 >= 0 ? max(p1 - a.window + 1, 0) : 0;
         const int sinks = a.sinks;
+        // ... and of the whole tile: its first row, and where its last row's window starts
+        const int tp0 = t.len - t.rows + c0 / grp, tp1 = t.len - t.rows + (c0 + ncol - 1) / grp;
+        const int tl1 = a.window && tp1 >= 0 ? max(tp1 - a.window + 1, 0) : 0;
 
         int ek, ev[NV];     // table entries of the next copies
         auto entries = [&](int i) {
@@ -716,30 +823,50 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
 #pragma unroll
         for (int d = 0; d < DT; d++) o[d] = f16_t{};
 
+        // A stage that some column of the tile does not see whole: what none of
+        // them sees may hold anything, and leaves V for zeros.  So do values
+        // that are not finite where some rows see them and others do not (0
+        // times one would reach those): true, and they are added one by one.
+        auto clean = [&](int base, int buf, uint64_t got) {
+            const int ql = a.window && tp0 >= 0 ? max(tp0 - a.window + 1, 0) : 0;
+            bool odd = false;
+#pragma unroll
+            for (int k = 0; k < NV; k++) {
+                const int g = k * AT_THREADS + tid, u = g / D;    // unit u of the stage: its row in K's order
+                const int row = U == 4 ? 4 * u : 32 * (u >> 2) + 16 * (u >> 1 & 1) + 4 * (u & 1);
+                const bool page = got >> row & 1;
+                uint4 &v = sv[buf][g];
+                uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int e = 0; e < U; e++) {
+                    const int p = base + u * U + e, sh = U == 4 ? 0 : 16 * (e & 1);
+                    uint32_t &x = w[U == 4 ? e % 4 : e / 2];
+                    const bool sees = page & (p <= tp1) & ((p >= ql) | (p < sinks));
+                    const bool bad = ((x >> sh & EXP) == EXP) & (tp0 != tp1);
+                    odd |= sees & bad;
+                    x = !sees | bad ? x & (U == 4 ? 0u : 0xffff0000u >> sh) : x;
+                }
+                v = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            return odd;
+        };
         // 32 positions from `base` on: half hf of the stage in `buf`
-        auto work_half = [&](int base, int buf, int hf, uint32_t got, auto masked) {
-            constexpr bool MASK = decltype(masked)::value;
+        auto work_half = [&](int base, int buf, int hf, uint32_t got, bool whole, bool odd) {
             f16_t sc = {};
 #pragma unroll
             for (int s = 0; s < DS; s++) sc = Ops::mul(sk[buf][(2 * s + h) * P + 32 * hf + col], q[s], sc);
-            // register r: position at(r) of these
-            auto at = [&](int r) { return U == 4 ? 8 * (r >> 2) + 4 * h + (r & 3) : 16 * (r >> 3) + 8 * h + (r & 7); };
-            bool page[NI];
-#pragma unroll
-            for (int r = 0; r < 16; r++) sc[r] *= unscale;
-            if (MASK) {
-#pragma unroll
-                for (int i = 0; i < NI; i++) page[i] = got >> (8 * (i * U >> 2) + 4 * h) & 1;   // a unit has one page
+            if (!whole) {
 #pragma unroll
                 for (int r = 0; r < 16; r++) {
                     const int p = base + at(r);
-                    if (!(page[r / U] && p <= pos && (p >= low || p < sinks))) sc[r] = -INFINITY;
+                    const bool page = got >> (8 * (r >> 2) + 4 * h + (r & 3)) & 1;
+                    sc[r] = page & (p <= pos) & ((p >= low) | (p < sinks)) ? sc[r] : -INFINITY;
                 }
             }
             float mx = sc[0];
 #pragma unroll
             for (int r = 1; r < 16; r++) mx = fmaxf(mx, sc[r]);
-            mx = fmaxf(m, half_max(mx));
+            mx = fmaxf(m, half_max(mx * unscale));
             if (__any(mx > m)) {
                 const float f = __builtin_amdgcn_exp2f(m - (mx == -INFINITY ? 0.0f : mx));
                 l *= f;
@@ -747,66 +874,56 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
                 for (int d = 0; d < DT; d++) o[d] *= f;
                 m = mx;
             }
-            const float sub = (m == -INFINITY ? 0.0f : m) - Ops::PSHIFT;
+            const float sub = Ops::PSHIFT - (m == -INFINITY ? 0.0f : m);
 #pragma unroll
             for (int r = 0; r < 16; r++) {
-                sc[r] = __builtin_amdgcn_exp2f(sc[r] - sub);
+                sc[r] = __builtin_amdgcn_exp2f(fmaf(sc[r], unscale, sub));
                 l += sc[r];
             }
 #pragma unroll
             for (int i = 0; i < NI; i++) {
-                float ps_[U];
+                float pr[U];
 #pragma unroll
-                for (int e = 0; e < U; e++) ps_[e] = sc[i * U + e];
-                const typename Ops::P pp = Ops::split(ps_);
-                const int unit = 32 / U * hf + 2 * i + h;
-                uint32_t keep[4];
-                if (MASK) {
-                    // what none of this wave's rows sees may hold anything
-                    uint32_t k1[U];
+                for (int e = 0; e < U; e++) pr[e] = sc[i * U + e];
+                const typename Ops::P pp = Ops::split(pr);
 #pragma unroll
-                    for (int e = 0; e < U; e++) {
-                        const int p = base + at(i * U + e);
-                        k1[e] = page[i] && p <= p1 && (p >= low0 || p < sinks) ? 0xffffffffu : 0u;
-                    }
+                for (int d = 0; d < DT; d++)
+                    o[d] = Ops::mul(sv[buf][(32 / U * hf + 2 * i + h) * D + 32 * d + col], pp, o[d]);
+            }
+            if (odd) {
+                // from the pool again: lane L holds a unit's dimension L of
+                // 64, and position (unit u, e) is register U (u / 2) + e of half u % 2
+#pragma unroll 1
+                for (int u = 0; u < 32 / U; u++) {
+                    const int p0u = base + u * U, g = kv_page(b, t.seq, p0u);
+                    if (g < 0) continue;
+#pragma unroll 1
+                    for (int d0 = 0; d0 < D; d0 += WAVE) {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(
+                            b.pool + (size_t)g * b.s.page_bytes + vbase +
+                            ((size_t)(t.head * (ps / U) + (p0u & (ps - 1)) / U) * D + min(d0 + lane, D - 1)) * 16);
+                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                    for (int w = 0; w < 4; w++)
-                        keep[w] = U == 4 ? k1[w % U] : (k1[(2 * w) % U] & 0xffffu) | (k1[(2 * w + 1) % U] & 0xffff0000u);
-                }
+                        for (int e = 0; e < U; e++) {
+                            const uint32_t bits = U == 4 ? w[e % 4] : w[e / 2] >> 16 * (e & 1) & 0xffffu;
+                            const bool sees = p0u + e <= pos && (p0u + e >= low || p0u + e < sinks);
+                            float pr = 0.0f;
 #pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    uint4 v = sv[buf][unit * D + 32 * d + col];
-                    if (MASK) {
-                        uint32_t w[4] = {v.x & keep[0], v.y & keep[1], v.z & keep[2], v.w & keep[3]};
-                        bool odd = false;
+                            for (int i = 0; i < NI; i++) pr = (u >> 1) == i ? sc[i * U + e] : pr;
+                            pr = __shfl(pr, (u & 1) * 32 + col, WAVE);
+                            for (uint64_t who = __ballot((bits & EXP) == EXP && d0 + lane < D); who; who &= who - 1) {
+                                const int L = __builtin_ctzll(who), dim = d0 + L;
+                                const float val = at_value(E{}, __builtin_amdgcn_readlane(bits, L));
+                                // dimension `dim` is register 4 (dim / 8 % 4) + dim % 4 of half dim / 4 % 2, tile dim / 32
+                                const float add = sees && (dim >> 2 & 1) == h ? pr * val : 0.0f;
 #pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            odd |= (w[k] & EXP) == EXP || (U == 8 && (w[k] & (EXP << 16)) == EXP << 16);
-                        if (p0 != p1 && __any(odd)) {
-                            // values that are not finite, one by one, as in the narrow form
-#pragma unroll
-                            for (int e = 0; e < U; e++) {
-                                const int sh = U == 4 ? 0 : 16 * (e & 1);
-                                const uint32_t bits = U == 4 ? w[e % 4] : (w[e / 2] >> sh) & 0xffffu;
-                                const bool bad = (bits & EXP) == EXP;
-                                for (uint64_t who = __ballot(bad); who; who &= who - 1) {
-                                    const int L = __builtin_ctzll(who);
-                                    const float val = at_value(E{}, __builtin_amdgcn_readlane(bits, L));
-                                    const float pr = __shfl(ps_[e], (L & 32) | col, WAVE);
-                                    const int p = base + (U == 4 ? 8 * i + 4 * (L >> 5) : 16 * i + 8 * (L >> 5)) + e;
-                                    const bool sees = p <= pos && (p >= low || p < sinks);
-                                    // dimension L % 32 is register 4 (dim / 8) + dim % 4 of half dim / 4 % 2
-                                    const float add = sees && (L >> 2 & 1) == h ? pr * val : 0.0f;
+                                for (int d = 0; d < DT; d++)
 #pragma unroll
                                     for (int r = 0; r < 16; r++)
-                                        o[d][r] += ((L >> 3 & 3) * 4 + (L & 3)) == r ? add : 0.0f;
-                                }
-                                if (bad) w[U == 4 ? e % 4 : e / 2] &= U == 4 ? 0u : 0xffff0000u >> sh;
+                                        o[d][r] += dim >> 5 == d && (dim >> 3 & 3) * 4 + (dim & 3) == r ? add : 0.0f;
                             }
                         }
-                        v = make_uint4(w[0], w[1], w[2], w[3]);
                     }
-                    o[d] = Ops::mul(v, pp, o[d]);
                 }
             }
         };
@@ -819,14 +936,15 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
                 entries(i + 2);
             }
             const int base = kv_base(t.span, i, SLOG);
+            bool odd = false;
+            if (!(base + P - 1 <= tp0 && (base >= tl1 || base + P <= sinks) && pages == ~(uint64_t)0))
+                odd = __syncthreads_or(clean(base, buf, pages));
 #pragma unroll 1
             for (int hf = 0; hf < HALVES; hf++) {
                 const int hb = base + 32 * hf;
                 if (!any || hb > p1 || (hb + 32 <= low0 && hb >= sinks)) continue;   // nobody's
                 const uint32_t got = (uint32_t)(pages >> 32 * hf);
-                const bool whole = hb + 31 <= p0 && (hb >= low1 || hb + 32 <= sinks) && got == 0xffffffffu;
-                if (whole) work_half(hb, buf, hf, got, std::false_type{});
-                else work_half(hb, buf, hf, got, std::true_type{});
+                work_half(hb, buf, hf, got, hb + 31 <= p0 && (hb >= low1 || hb + 32 <= sinks) && got == 0xffffffffu, odd);
             }
             pages = pages_next;
         }
@@ -947,7 +1065,7 @@ __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttn a, const AtJoi
 template <class E, int D>
 static void attn_launch_d(qq_ctx *ctx, const qq_kv *kv, const KvBatch &b, const KvAttn &a)
 {
-    const size_t shm = (size_t)(b.n_seqs + 1) * sizeof(uint64_t);
+    const size_t shm = at_plan_bytes(b);
     AtJoin *joins = reinterpret_cast<AtJoin *>(kv->work);
     // Many rows a sequence: more than two narrow tiles' columns.
     const bool wide = b.row_start && (int64_t)b.n_rows * a.group > (int64_t)2 * AT_COLS * b.n_seqs;

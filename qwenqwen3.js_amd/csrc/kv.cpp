@@ -438,7 +438,7 @@ int qq_kv_attn_dev(qq_ctx *ctx, qq_kv *kv, int layer, const qq_kv_batch *batch, 
     if (!q_dev || !out_dev) return set_error(ctx, "kv_attn: NULL buffer");
     // steps of 16 positions, at the most that the tables allow: their count in 50 bits (kv_plan.h)
     const uint64_t tiles = ((uint64_t)batch->n_rows * n_heads + 15) / 16 + (uint64_t)batch->n_seqs * kv->s.n_kv_heads;
-    if (tiles * ((uint64_t)batch->table_stride * kv->s.page_size / 16) >> 50)
+    if ((uint64_t)batch->n_rows * n_heads > 1u << 30 || tiles * ((uint64_t)batch->table_stride * kv->s.page_size / 16) >> 50)
         return set_error(ctx, "kv_attn: %d rows of %d heads over tables of %d pages", batch->n_rows, n_heads,
                          batch->table_stride);
     if (overlap(q_dev, out_dev, (size_t)batch->n_rows * n_heads * kv->s.head_dim * sizeof(float)))
