@@ -55,6 +55,7 @@ __host__ __device__ constexpr int at_per_cu(int dim) { return dim == 32 ? 4 : di
 static int attn_parts(const qq_ctx *ctx, int dim) { return std::min(ctx->num_cus * at_per_cu(dim), 4095); }
 // The form for many rows: 128 columns, 32 a wave
 constexpr int AW_COLS = 128;
+constexpr int AW_LEAD = 2;
 constexpr int AW_PER_CU = 2;
 static int wide_parts(const qq_ctx *ctx) { return std::min(ctx->num_cus * AW_PER_CU, 4095); }
 
@@ -72,6 +73,27 @@ size_t kv_attn_work_bytes(const qq_ctx *ctx, const KvShape &s)
     const size_t narrow = sizeof(AtJoin) + 2 * attn_slot(AT_COLS, s.head_dim) * sizeof(float);
     const size_t wide = sizeof(AtJoin) + 2 * attn_slot(AW_COLS, s.head_dim) * sizeof(float);
     return std::max(attn_parts(ctx, s.head_dim) * narrow, wide_parts(ctx) * wide);
+}
+
+// Two fp32 rounded to fp16 in one register, and what rounding left of either
+// (by the instructions: the compiler converts twice to take the pair apart).
+__device__ __forceinline__ uint32_t f16_pair(float a, float b)
+{
+    uint32_t r;
+    asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ float f16_rest0(uint32_t h, float x)
+{
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    return r;
+}
+__device__ __forceinline__ float f16_rest1(uint32_t h, float x)
+{
+    float r;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+    return r;
 }
 
 // ---- operands by cache type: q's planes, a step's probabilities -------------------
@@ -154,11 +176,15 @@ struct AtOps<KvF16> {
     typedef Q P;
     static __device__ __forceinline__ Q split(const float (&x)[8])
     {
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            h[i] = f16_pair(x[2 * i], x[2 * i + 1]);
+            l[i] = f16_pair(f16_rest0(h[i], x[2 * i]), f16_rest1(h[i], x[2 * i + 1]));
+        }
         Q q;
-#pragma unroll
-        for (int i = 0; i < 8; i++) q.h[i] = (_Float16)x[i];
-#pragma unroll
-        for (int i = 0; i < 8; i++) q.l[i] = (_Float16)fmaf(-1.0f, (float)q.h[i], x[i]);
+        q.h = __builtin_bit_cast(h8_t, make_uint4(h[0], h[1], h[2], h[3]));
+        q.l = __builtin_bit_cast(h8_t, make_uint4(l[0], l[1], l[2], l[3]));
         return q;
     }
     static __device__ __forceinline__ f4_t mul(const uint4 &a, const Q &q, f4_t c)
@@ -233,7 +259,7 @@ __device__ __forceinline__ float half_sum(float v)
 struct AtTile {
     int seq, head, t;        // sequence, key/value head, column tile
     int row0, rows, len;     // the sequence's new rows and length
-    uint64_t start;          // the tile's first step among the call's (AT_LEAD of them ahead of its own)
+    uint64_t start;          // the tile's first step among the call's (LEAD of them ahead of its own)
     KvSpan span;
 };
 
@@ -276,7 +302,7 @@ __device__ __forceinline__ V at_scan(V v, V &total, uint64_t *red)
     return off;
 }
 
-template <bool ROWS, int COLS, int SLOG, int NT>
+template <bool ROWS, int COLS, int LEAD, int SLOG, int NT>
 struct AtWork {
     const KvBatch &b;
     const KvAttn &a;
@@ -358,7 +384,7 @@ struct AtWork {
             int seq, t;
             place(g0, seq, t);
             for (int g = g0;;) {
-                sum += span(len[seq], ROWS ? rows[seq] : 1, t).n + AT_LEAD;
+                sum += span(len[seq], ROWS ? rows[seq] : 1, t).n + LEAD;
                 if (++g == g1) break;
                 next(seq, t);
             }
@@ -390,8 +416,8 @@ struct AtWork {
             t.len = uni(len[t.seq]);
             t.rows = ROWS ? uni(rows[t.seq]) : 1;
             t.span = span(t.len, t.rows, t.t);
-            if (r < start + AT_LEAD + t.span.n) break;
-            start += AT_LEAD + t.span.n;
+            if (r < start + LEAD + t.span.n) break;
+            start += LEAD + t.span.n;
             next(t.seq, t.t);
         }
         t.row0 = ROWS ? uni(row0[t.seq]) : t.seq;
@@ -416,7 +442,7 @@ __global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBat
     __shared__ __align__(16) float so[AT_WAVES][AT_COLS][LDO];
     __shared__ float sm[AT_WAVES][AT_COLS], sl[AT_WAVES][AT_COLS];
     __shared__ AtPlan<AT_THREADS> plan;
-    AtWork<ROWS, AT_COLS, SLOG, AT_THREADS> wk(b, a, plan, seqs);
+    AtWork<ROWS, AT_COLS, AT_LEAD, SLOG, AT_THREADS> wk(b, a, plan, seqs);
     float *const work = reinterpret_cast<float *>(joins + gridDim.x);
     const uint64_t W = wk.plan();
     const uint32_t n = kv_parts(W, gridDim.x, AT_LEAST);
@@ -707,12 +733,13 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
     constexpr int KU = D / U * P, VU = P / U * D;          // units of a stage
     constexpr int NK = KU / AT_THREADS, NV = VU / AT_THREADS;
     constexpr int DS = D / (2 * U), DT = D / 32, HALVES = P / 32, NI = 16 / U;
+    constexpr int JH = HALVES == 2 && D <= 64 ? 2 : 1;
     constexpr uint32_t EXP = U == 4 ? 0x7f800000u : Ops::PSHIFT != 0.0f ? 0x7c00u : 0x7f80u;
     static_assert(KU % AT_THREADS == 0 && VU % AT_THREADS == 0, "copies by whole workgroups");
     extern __shared__ int seqs[];
     __shared__ __align__(16) uint4 sk[2][KU], sv[2][VU];
     __shared__ AtPlan<AT_THREADS> plan;
-    AtWork<true, AW_COLS, SLOG, AT_THREADS> wk(b, a, plan, seqs);
+    AtWork<true, AW_COLS, AW_LEAD, SLOG, AT_THREADS> wk(b, a, plan, seqs);
     float *const work = reinterpret_cast<float *>(joins + gridDim.x);
     const uint64_t W = wk.plan();
     const uint32_t n = kv_parts(W, gridDim.x, AT_LEAST);
@@ -731,13 +758,14 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
     // the position that this lane copies of K (unit tid of AT_THREADS: position tid % P in the rows' order)
     const int kr = tid % P % 32;
     const int kp = tid % P / 32 * 32 + (U == 4 ? kr : 16 * (kr >> 4) + 8 * (kr >> 2 & 1) + 4 * (kr >> 3 & 1) + (kr & 3));
+    const uint32_t koff = (uint32_t)(tid / P * ps + kp) * 16;   // ... and its place behind the first one's
     // the position of register r among 32
     auto at = [&](int r) { return U == 4 ? 8 * (r >> 2) + 4 * h + (r & 3) : 16 * (r >> 3) + 8 * h + (r & 7); };
     const uint32_t lk = lds_u32(&sk[0][wave * WAVE]), lv = lds_u32(&sv[0][wave * WAVE]);
 
     for (uint64_t x = x0; x < x1;) {
         const AtTile t = wk.find(x);
-        const uint64_t own = t.start + AT_LEAD, tend = own + t.span.n;
+        const uint64_t own = t.start + AW_LEAD, tend = own + t.span.n;
         x = tend;
         if (own >= x1) break;    // the next workgroup's
         const int i0 = x0 > own ? (int)(x0 - own) : 0;
@@ -757,16 +785,36 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
         const int tp0 = t.len - t.rows + c0 / grp, tp1 = t.len - t.rows + (c0 + ncol - 1) / grp;
         const int tl1 = a.window && tp1 >= 0 ? max(tp1 - a.window + 1, 0) : 0;
 
-        int ek, ev[NV];     // table entries of the next copies
+        // Table entries of the next copies, and the copies (which return which
+        // of the stage's positions, in the rows' order, have a page).  Pages of
+        // a stage or more: one entry, and lanes that differ by a constant.
+        const bool one = ps >= P;
+        int ek, ev[NV];
         auto entries = [&](int i) {
             const int base = kv_base(t.span, min(i, i1 - 1), SLOG);
+            if (one) {
+                ek = kv_entry(b, t.seq, base);
+                return;
+            }
             ek = kv_entry(b, t.seq, base + kp);
 #pragma unroll
             for (int k = 0; k < NV; k++) ev[k] = kv_entry(b, t.seq, base + (k * AT_THREADS + tid) / D * U);
         };
-        // (returns which of the stage's positions, in the rows' order, have a page)
         auto copy = [&](int i, int buf) -> uint64_t {
             const int base = kv_base(t.span, i, SLOG);
+            if (one) {
+                const int g = uni(kv_page_of(b, base, ek)), slot = base & (ps - 1);
+                const char *page = b.pool + (size_t)max(g, 0) * b.s.page_bytes;
+                const char *kb = page + ((size_t)t.head * (D / U) * ps + slot) * 16;
+                const char *vb = page + vbase + ((size_t)t.head * ps + slot) * (D / U) * 16;
+#pragma unroll
+                for (int k = 0; k < NK; k++)
+                    dma16s(koff, kb + (size_t)k * (AT_THREADS / P) * ps * 16, lk + (buf * KU + k * AT_THREADS) * 16);
+#pragma unroll
+                for (int k = 0; k < NV; k++)
+                    dma16s(tid * 16, vb + k * AT_THREADS * 16, lv + (buf * VU + k * AT_THREADS) * 16);
+                return g >= 0 ? ~(uint64_t)0 : 0;
+            }
             const int at = base + kp, kg = kv_page_of(b, at, ek);
             const char *src = b.pool + (size_t)max(kg, 0) * b.s.page_bytes +
                               ((size_t)(t.head * (D / U) + tid / P) * ps + (at & (ps - 1))) * 16;
@@ -850,22 +898,33 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
             }
             return odd;
         };
-        // 32 positions from `base` on: half hf of the stage in `buf`
-        auto work_half = [&](int base, int buf, int hf, uint32_t got, bool whole, bool odd) {
-            f16_t sc = {};
+        // 32 JH positions from `base` on: halves hf .. of the stage in `buf`.
+        // (Together where registers allow: the sums of one half then run
+        // beside the exponentials of the other.)
+        auto work_half = [&](int base, int buf, int hf, uint64_t got, bool whole, bool odd) {
+            f16_t sc[JH];
 #pragma unroll
-            for (int s = 0; s < DS; s++) sc = Ops::mul(sk[buf][(2 * s + h) * P + 32 * hf + col], q[s], sc);
+            for (int g = 0; g < JH; g++) sc[g] = f16_t{};
+#pragma unroll
+            for (int s = 0; s < DS; s++)
+#pragma unroll
+                for (int g = 0; g < JH; g++)
+                    sc[g] = Ops::mul(sk[buf][(2 * s + h) * P + 32 * (hf + g) + col], q[s], sc[g]);
             if (!whole) {
 #pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int p = base + at(r);
-                    const bool page = got >> (8 * (r >> 2) + 4 * h + (r & 3)) & 1;
-                    sc[r] = page & (p <= pos) & ((p >= low) | (p < sinks)) ? sc[r] : -INFINITY;
-                }
-            }
-            float mx = sc[0];
+                for (int g = 0; g < JH; g++)
 #pragma unroll
-            for (int r = 1; r < 16; r++) mx = fmaxf(mx, sc[r]);
+                    for (int r = 0; r < 16; r++) {
+                        const int p = base + 32 * g + at(r);
+                        const bool page = (uint32_t)(got >> 32 * g) >> (8 * (r >> 2) + 4 * h + (r & 3)) & 1;
+                        sc[g][r] = page & (p <= pos) & ((p >= low) | (p < sinks)) ? sc[g][r] : -INFINITY;
+                    }
+            }
+            float mx = sc[0][0];
+#pragma unroll
+            for (int g = 0; g < JH; g++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) mx = fmaxf(mx, sc[g][r]);
             mx = fmaxf(m, half_max(mx * unscale));
             if (__any(mx > m)) {
                 const float f = __builtin_amdgcn_exp2f(m - (mx == -INFINITY ? 0.0f : mx));
@@ -876,25 +935,28 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
             }
             const float sub = Ops::PSHIFT - (m == -INFINITY ? 0.0f : m);
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                sc[r] = __builtin_amdgcn_exp2f(fmaf(sc[r], unscale, sub));
-                l += sc[r];
-            }
+            for (int g = 0; g < JH; g++) {
 #pragma unroll
-            for (int i = 0; i < NI; i++) {
-                float pr[U];
+                for (int r = 0; r < 16; r++) {
+                    sc[g][r] = __builtin_amdgcn_exp2f(fmaf(sc[g][r], unscale, sub));
+                    l += sc[g][r];
+                }
 #pragma unroll
-                for (int e = 0; e < U; e++) pr[e] = sc[i * U + e];
-                const typename Ops::P pp = Ops::split(pr);
+                for (int i = 0; i < NI; i++) {
+                    float pr[U];
 #pragma unroll
-                for (int d = 0; d < DT; d++)
-                    o[d] = Ops::mul(sv[buf][(32 / U * hf + 2 * i + h) * D + 32 * d + col], pp, o[d]);
+                    for (int e = 0; e < U; e++) pr[e] = sc[g][i * U + e];
+                    const typename Ops::P pp = Ops::split(pr);
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+                        o[d] = Ops::mul(sv[buf][(32 / U * (hf + g) + 2 * i + h) * D + 32 * d + col], pp, o[d]);
+                }
             }
             if (odd) {
                 // from the pool again: lane L holds a unit's dimension L of
                 // 64, and position (unit u, e) is register U (u / 2) + e of half u % 2
 #pragma unroll 1
-                for (int u = 0; u < 32 / U; u++) {
+                for (int u = 0; u < 32 * JH / U; u++) {
                     const int p0u = base + u * U, g = kv_page(b, t.seq, p0u);
                     if (g < 0) continue;
 #pragma unroll 1
@@ -909,7 +971,7 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
                             const bool sees = p0u + e <= pos && (p0u + e >= low || p0u + e < sinks);
                             float pr = 0.0f;
 #pragma unroll
-                            for (int i = 0; i < NI; i++) pr = (u >> 1) == i ? sc[i * U + e] : pr;
+                            for (int i = 0; i < NI * JH; i++) pr = (u >> 1) == i ? sc[i / NI][i % NI * U + e] : pr;
                             pr = __shfl(pr, (u & 1) * 32 + col, WAVE);
                             for (uint64_t who = __ballot((bits & EXP) == EXP && d0 + lane < D); who; who &= who - 1) {
                                 const int L = __builtin_ctzll(who), dim = d0 + L;
@@ -940,11 +1002,11 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
             if (!(base + P - 1 <= tp0 && (base >= tl1 || base + P <= sinks) && pages == ~(uint64_t)0))
                 odd = __syncthreads_or(clean(base, buf, pages));
 #pragma unroll 1
-            for (int hf = 0; hf < HALVES; hf++) {
-                const int hb = base + 32 * hf;
-                if (!any || hb > p1 || (hb + 32 <= low0 && hb >= sinks)) continue;   // nobody's
-                const uint32_t got = (uint32_t)(pages >> 32 * hf);
-                work_half(hb, buf, hf, got, hb + 31 <= p0 && (hb >= low1 || hb + 32 <= sinks) && got == 0xffffffffu, odd);
+            for (int hf = 0; hf < HALVES; hf += JH) {
+                const int hb = base + 32 * hf, he = hb + 32 * JH;
+                if (!any || hb > p1 || (he <= low0 && hb >= sinks)) continue;   // nobody's
+                const uint64_t all = JH == 2 ? ~(uint64_t)0 : 0xffffffffu, got = pages >> 32 * hf & all;
+                work_half(hb, buf, hf, got, he - 1 <= p0 && (hb >= low1 || he <= sinks) && got == all, odd);
             }
             pages = pages_next;
         }
@@ -994,7 +1056,7 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
 template <int COLS, int D, int JC>
 __global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttn a, const AtJoin *__restrict__ joins)
 {
-    constexpr int LN = D / 4, CL = 256 / (LN * JC), AHEAD = 8;
+    constexpr int LN = D / 4, CL = 256 / (LN * JC), AHEAD = JC == 1 ? 8 : 2;
     __shared__ float sms[JC][CL], sls[JC][CL];
     __shared__ __align__(16) f4_t sos[JC][CL][LN];
     const AtJoin t = joins[blockIdx.x];
