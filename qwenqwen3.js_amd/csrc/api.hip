@@ -124,7 +124,7 @@ static const char *const kKernelNames[K_COUNT] = {
     "cast_f16",         "mfma_gateup",    "mfma_down",      "stream_gateup", "stream_down",
     "rmsnorm", "lfm2_embed", "lfm2_matvec", "lfm2_attention", "route_dispatch",
     "row_inv",
-    "kv_store", "kv_attention", "kv_join", "kv_pages",
+    "kv_store", "kv_attention", "kv_pages",
 };
 
 // After a timed-out call: clear the error word and move the epoch on by

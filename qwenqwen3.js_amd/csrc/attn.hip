@@ -30,7 +30,8 @@
 // its first loads and its end cost a workgroup.  A workgroup's waves take its
 // steps in turn and join in LDS; what a cut separates goes to the workspace,
 // two slots a workgroup (a tile it goes on with from the workgroup before it,
-// and one it leaves to the next), and a second launch joins those.
+// and one it leaves to the next), and the last workgroup to bring a tile's
+// part joins them, in the order of the parts.
 #include "kv_device.h"
 #include "kv_plan.h"
 
@@ -49,30 +50,30 @@ constexpr int AT_WAVES = 4;      // waves of a workgroup
 constexpr int AT_THREADS = AT_WAVES * WAVE;
 constexpr int AT_LEAD = 4;       // steps that a tile's beginning and end are worth
 constexpr int AT_LEAST = 4;      // steps a part has at least
+constexpr int AT_GROUP = 16;     // parts of a tile that one workgroup joins
 // workgroups a CU holds, by registers: a wave keeps two steps of values and one of keys, q's planes and the sums
-__host__ __device__ constexpr int at_per_cu(int dim) { return dim == 32 ? 4 : dim == 64 ? 3 : 2; }
+__host__ __device__ constexpr int at_per_cu(int dim) { return dim <= 64 ? 3 : 2; }
 
 static int attn_parts(const qq_ctx *ctx, int dim) { return std::min(ctx->num_cus * at_per_cu(dim), 4095); }
 // The form for many rows: 128 columns, 32 a wave
 constexpr int AW_COLS = 128;
 constexpr int AW_LEAD = 2;
+constexpr int AW_GROUP = 8;
 constexpr int AW_PER_CU = 2;
 static int wide_parts(const qq_ctx *ctx) { return std::min(ctx->num_cus * AW_PER_CU, 4095); }
 
-// The workspace: what every workgroup leaves to the join (count 0: nothing),
-// then its slots, in floats: the columns' D sums, their maxima and sums of
-// probabilities.
-struct AtJoin {
-    int count;                   // workgroups that share the tile, this one the first
-    int row0, c0, ncol, head;    // its sequence's first row, its columns, its key/value head
-    int pad[3];
-};
-__host__ __device__ constexpr int attn_slot(int cols, int dim) { return cols * (dim + 2); }
+// The workspace: counters of arrived parts, zero between launches (who finds
+// its tile complete clears them), three for every workgroup; then its slots,
+// in words of two floats: the columns' D sums (two planes of half of every
+// four, or each thread's), then maximum and sum of probabilities of a column,
+// or of each thread's.
+__host__ __device__ constexpr int attn_slot(int cols, int dim) { return cols * (dim / 2 + 2); }
+__host__ __device__ constexpr size_t attn_counters(int parts) { return ((size_t)parts * 3 + 63) / 64 * 64; }
 size_t kv_attn_work_bytes(const qq_ctx *ctx, const KvShape &s)
 {
-    const size_t narrow = sizeof(AtJoin) + 2 * attn_slot(AT_COLS, s.head_dim) * sizeof(float);
-    const size_t wide = sizeof(AtJoin) + 2 * attn_slot(AW_COLS, s.head_dim) * sizeof(float);
-    return std::max(attn_parts(ctx, s.head_dim) * narrow, wide_parts(ctx) * wide);
+    const int narrow = attn_parts(ctx, s.head_dim), wide = wide_parts(ctx);
+    return 4 * attn_counters(std::max(narrow, wide)) + 8 * std::max((size_t)narrow * 2 * attn_slot(AT_COLS, s.head_dim),
+                                                                   (size_t)wide * 2 * attn_slot(AW_COLS, s.head_dim));
 }
 
 // Two fp32 rounded to fp16 in one register, and what rounding left of either
@@ -426,12 +427,80 @@ struct AtWork {
     }
 };
 
+// ---- tiles in parts -------------------------------------------------------------------
+
+// Slots are written through to memory and read from there (relaxed atomics of
+// device scope), so that a workgroup on another XCD needs no cache written
+// back or thrown away before it reads one: with fences in their place 64
+// ragged sequences took 127 us, not 57.
+// A slot is words of two floats, consecutive lanes' words side by side.
+__device__ __forceinline__ void slot_put(uint64_t *p, float a, float b)
+{
+    __hip_atomic_store(p, (uint64_t)__float_as_uint(b) << 32 | __float_as_uint(a), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 slot_get(const uint64_t *p)
+{
+    const uint64_t v = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float((uint32_t)v), __uint_as_float((uint32_t)(v >> 32)));
+}
+
+// A tile's parts w0 .. w0 + count - 1, this workgroup's the k-th.  Up to GROUP
+// are joined by whoever brings the last; more in groups of so many first, by
+// the last of each, into the group's first slot.
+struct AtSplit {
+    uint32_t *counters;
+    uint64_t *slots;
+    uint32_t parts, w0;
+    int k, count, slot;     // slot: words of one
+
+    __device__ __forceinline__ AtSplit(uint32_t *work, uint32_t grid, int slot_, uint64_t W, uint32_t n, uint32_t part,
+                                       uint64_t own, uint64_t tend)
+        : counters(work), slots(reinterpret_cast<uint64_t *>(work + attn_counters(grid))), parts(grid), slot(slot_)
+    {
+        w0 = kv_part(W, n, own);
+        count = (int)(kv_part(W, n, tend - 1) - w0) + 1;
+        k = (int)(part - w0);
+    }
+    __device__ __forceinline__ uint64_t *at(int i) const
+    {
+        return slots + (size_t)(2 * (w0 + i) + (i == 0)) * slot;
+    }
+    // Whether this workgroup is the last of `all` to count itself in: every
+    // wave's stores to the slot are acknowledged first.
+    __device__ __forceinline__ bool last(uint32_t *counter, int all, uint32_t *said) const
+    {
+        wait_vm<0>();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            const uint32_t before = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if ((int)before == all - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            *said = (int)before == all - 1;
+        }
+        __syncthreads();
+        return *said;
+    }
+    // join(first, step, number, into): the parts first, first + step, ... into a slot, or the result (NULL)
+    template <int GROUP, class F>
+    __device__ __forceinline__ void bring(uint32_t *said, F join) const
+    {
+        if (count <= GROUP) {
+            if (last(counters + w0, count, said)) join(0, 1, count, nullptr);
+            return;
+        }
+        const int g = k / GROUP, first = g * GROUP, size = min(GROUP, count - first);
+        // (a workgroup may be the first of one tile and in the middle of another)
+        if (!last(counters + (g == 0 ? parts : 2 * parts) + w0 + first, size, said)) return;
+        join(first, 1, size, at(first));
+        if (last(counters + w0, (count + GROUP - 1) / GROUP, said)) join(0, GROUP, (count + GROUP - 1) / GROUP, nullptr);
+    }
+};
+
 // ---- the kernel ---------------------------------------------------------------------
 
 // ROWS: a tile's columns may be several rows, that see different positions.
 template <class E, int D, bool ROWS>
-__global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBatch b, KvAttn a,
-                                                                          AtJoin *__restrict__ joins)
+__global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBatch b, KvAttn a, uint32_t *work)
 {
     typedef AtOps<E> Ops;
     constexpr int U = E::U, TK = U / 4, DS = D / (4 * U), DT = D / 16;
@@ -443,13 +512,12 @@ __global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBat
     __shared__ float sm[AT_WAVES][AT_COLS], sl[AT_WAVES][AT_COLS];
     __shared__ AtPlan<AT_THREADS> plan;
     AtWork<ROWS, AT_COLS, AT_LEAD, SLOG, AT_THREADS> wk(b, a, plan, seqs);
-    float *const work = reinterpret_cast<float *>(joins + gridDim.x);
+    __shared__ uint32_t said;
     const uint64_t W = wk.plan();
     const uint32_t n = kv_parts(W, gridDim.x, AT_LEAST);
     // (no steps, or fewer parts than workgroups: none for this one)
     const uint64_t x0 = W && blockIdx.x < n ? kv_cut(W, n, blockIdx.x) : 0;
     const uint64_t x1 = W && blockIdx.x < n ? kv_cut(W, n, blockIdx.x + 1) : 0;
-    int left_count = 0, left_row0 = 0, left_c0 = 0, left_ncol = 0, left_head = 0;   // this workgroup's AtJoin
 
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = uni(tid / WAVE);
     const int col = lane & 15, j = lane >> 4;
@@ -671,9 +739,19 @@ __global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBat
 #pragma unroll
         for (int d = 0; d < DT; d++) *reinterpret_cast<f4_t *>(&so[wave][col][16 * d + 4 * j]) = o[d];
         __syncthreads();
-        // whole: the result; else this workgroup's slot for a tile that began before it, or that goes on behind it
+        // whole: the result; else this workgroup's part of it
         const bool mine = i0 == 0 && i1 == t.span.n;
-        float *slot = work + (size_t)(2 * blockIdx.x + (i0 == 0 ? 1 : 0)) * attn_slot(AT_COLS, D);
+        const AtSplit split(work, gridDim.x, attn_slot(AT_COLS, D), W, n, blockIdx.x, own, tend);
+        auto result = [&](int c, int d, const f4_t &sum, float L) {
+            const int row = t.row0 + (c0 + c) / grp, head = t.head * grp + (c0 + c) % grp;
+            // nothing seen: L = 0 and a sum of zeros
+            *reinterpret_cast<f4u_t *>(a.out + ((size_t)row * nh + head) * D + d) = L == 0.0f ? sum : sum / L;
+        };
+        auto keep = [&](uint64_t *slot, int c, int d, const f4_t &sum, float M, float L) {
+            slot_put(slot + (c * D + d) / 4, sum[0], sum[1]);
+            slot_put(slot + (AT_COLS * D + c * D + d) / 4, sum[2], sum[3]);
+            if (d == 0) slot_put(slot + AT_COLS * D / 2 + c, M, L);
+        };
         for (int e = tid; e < ncol * (D / 4); e += AT_THREADS) {
             const int c = e / (D / 4), d = e % (D / 4) * 4;
             float M = sm[0][c];
@@ -688,29 +766,52 @@ __global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBat
                 sum += *reinterpret_cast<const f4_t *>(&so[w][c][d]) * r;
                 L += sl[w][c] * r;
             }
-            if (mine) {
-                const int row = t.row0 + (c0 + c) / grp, head = t.head * grp + (c0 + c) % grp;
-                // nothing seen: L = 0 and a sum of zeros
-                const f4_t out = L == 0.0f ? sum : sum / L;
-                *reinterpret_cast<f4u_t *>(a.out + ((size_t)row * nh + head) * D + d) = out;
-            } else {
-                *reinterpret_cast<f4_t *>(slot + c * D + d) = sum;
-                if (d == 0) {
-                    slot[AT_COLS * D + c] = M;
-                    slot[AT_COLS * (D + 1) + c] = L;
+            if (mine) result(c, d, sum, L);
+            else keep(split.at(split.k), c, d, sum, M, L);
+        }
+        if (!mine)
+            split.template bring<AT_GROUP>(&said, [&](int first, int by, int num, uint64_t *into) {
+                for (int e0 = 0; e0 < ncol * (D / 4); e0 += AT_THREADS) {
+                    // (threads behind the last element do its work and store nothing)
+                    const int e = min(e0 + tid, ncol * (D / 4) - 1), c = e / (D / 4), d = e % (D / 4) * 4;
+                    constexpr int AHEAD = 8;
+                    float M = -INFINITY, L = 0.0f;
+                    f4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
+                    for (int k = 0; k < num; k += AHEAD) {
+                        float m[AHEAD], l[AHEAD];
+                        f4_t v[AHEAD];
+#pragma unroll
+                        for (int u = 0; u < AHEAD; u++) {
+                            const uint64_t *s = split.at(first + by * min(k + u, num - 1));
+                            const float2 ml = slot_get(s + AT_COLS * D / 2 + c);
+                            const float2 x = slot_get(s + (c * D + d) / 4), y = slot_get(s + (AT_COLS * D + c * D + d) / 4);
+                            m[u] = ml.x;
+                            l[u] = ml.y;
+                            v[u] = f4_t{x.x, x.y, y.x, y.y};
+                        }
+                        float top = M;
+#pragma unroll
+                        for (int u = 0; u < AHEAD; u++) top = fmaxf(top, m[u]);
+                        const float ts = top == -INFINITY ? 0.0f : top, r = __builtin_amdgcn_exp2f(M - ts);
+                        sum *= r;
+                        L *= r;
+#pragma unroll
+                        for (int u = 0; u < AHEAD; u++)
+                            if (k + u < num) {
+                                const float w = __builtin_amdgcn_exp2f(m[u] - ts);
+                                sum += v[u] * w;
+                                L += l[u] * w;
+                            }
+                        M = top;
+                    }
+                    __syncthreads();    // `into` is one of these slots
+                    if (e0 + tid >= ncol * (D / 4)) continue;
+                    if (into) keep(into, c, d, sum, M, L);
+                    else result(c, d, sum, L);
                 }
-            }
-        }
-        if (i0 == 0 && !mine) {
-            left_count = (int)(kv_part(W, n, tend - 1) - blockIdx.x) + 1;
-            left_row0 = t.row0;
-            left_c0 = c0;
-            left_ncol = ncol;
-            left_head = t.head;
-        }
+            });
         __syncthreads();   // LDS is used again
     }
-    if (tid == 0) joins[blockIdx.x] = AtJoin{left_count, left_row0, left_c0, left_ncol, left_head, {0, 0, 0}};
 }
 
 // ---- many rows ----------------------------------------------------------------------
@@ -725,8 +826,7 @@ __global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBat
 // + 4 (a % 2) + b of 16-bit types, m of fp32: the scores of a lane's half h
 // then are those of whole units of V.
 template <class E, int D>
-__global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvBatch b, KvAttn a,
-                                                                            AtJoin *__restrict__ joins)
+__global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvBatch b, KvAttn a, uint32_t *work)
 {
     typedef AtOps<E> Ops;
     constexpr int U = E::U, P = U == 4 ? 32 : 64, SLOG = U == 4 ? 5 : 6;
@@ -740,7 +840,7 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
     __shared__ __align__(16) uint4 sk[2][KU], sv[2][VU];
     __shared__ AtPlan<AT_THREADS> plan;
     AtWork<true, AW_COLS, AW_LEAD, SLOG, AT_THREADS> wk(b, a, plan, seqs);
-    float *const work = reinterpret_cast<float *>(joins + gridDim.x);
+    __shared__ uint32_t said;
     const uint64_t W = wk.plan();
     const uint32_t n = kv_parts(W, gridDim.x, AT_LEAST);
     // parts in a row on one XCD (workgroups go to the eight in turn): they read the same keys and values
@@ -748,7 +848,6 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
     const uint32_t part = gridDim.x % 8 ? blockIdx.x : blockIdx.x % 8 * per + blockIdx.x / 8;
     const uint64_t x0 = W && part < n ? kv_cut(W, n, part) : 0;
     const uint64_t x1 = W && part < n ? kv_cut(W, n, part + 1) : 0;
-    int left_count = 0, left_row0 = 0, left_c0 = 0, left_ncol = 0, left_head = 0;   // this workgroup's AtJoin
 
     const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = uni(tid / WAVE);
     const int col = lane & 31, h = lane >> 5;
@@ -792,11 +891,7 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
         int ek, ev[NV];
         auto entries = [&](int i) {
             const int base = kv_base(t.span, min(i, i1 - 1), SLOG);
-            if (one) {
-                ek = kv_entry(b, t.seq, base);
-                return;
-            }
-            ek = kv_entry(b, t.seq, base + kp);
+            ek = kv_entry(b, t.seq, base + kp);   // (no branch: what is loaded under one is waited for at its end)
 #pragma unroll
             for (int k = 0; k < NV; k++) ev[k] = kv_entry(b, t.seq, base + (k * AT_THREADS + tid) / D * U);
         };
@@ -1011,141 +1106,75 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
             pages = pages_next;
         }
 
-        // ---- results, or this workgroup's slot ----
+        // ---- results, or this workgroup's part of them ----
         l = half_sum(l);
-        const bool mine = i0 == 0 && i1 == t.span.n;
-        if (wave * 32 + col < ncol) {
-            const int c = wave * 32 + col;
-            if (mine) {
-                float *dst = a.out + ((size_t)(t.row0 + cr) * nh + t.head * grp + cc % grp) * D;
+        const int c = wave * 32 + col;      // this lane's column, dimensions 32 d + 8 k + 4 h ..
+        auto result = [&](const f16_t (&v)[DT], float L) {
+            float *dst = a.out + ((size_t)(t.row0 + cr) * nh + t.head * grp + cc % grp) * D;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const f4_t x = {v[d][4 * k], v[d][4 * k + 1], v[d][4 * k + 2], v[d][4 * k + 3]};
+                    *reinterpret_cast<f4u_t *>(dst + 32 * d + 8 * k + 4 * h) = L == 0.0f ? x : x / L;
+                }
+        };
+        auto keep = [&](uint64_t *slot, const f16_t (&v)[DT], float M, float L) {
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) slot_put(slot + (8 * d + k) * AT_THREADS + tid, v[d][2 * k], v[d][2 * k + 1]);
+            slot_put(slot + 8 * DT * AT_THREADS + tid, M, L);
+        };
+        if (i0 == 0 && i1 == t.span.n) {
+            if (c < ncol) result(o, l);
+            continue;
+        }
+        const AtSplit split(work, gridDim.x, attn_slot(AW_COLS, D), W, n, part, own, tend);
+        if (c < ncol) keep(split.at(split.k), o, m, l);
+        split.template bring<AW_GROUP>(&said, [&](int first, int by, int num, uint64_t *into) {
+            if (c >= ncol) return;
+            float M = -INFINITY, L = 0.0f;
+            f16_t sum[DT];
+#pragma unroll
+            for (int d = 0; d < DT; d++) sum[d] = f16_t{};
+            for (int i = 0; i < num; i++) M = fmaxf(M, slot_get(split.at(first + by * i) + 8 * DT * AT_THREADS + tid).x);
+            const float ms = M == -INFINITY ? 0.0f : M;
+            for (int i = 0; i < num; i++) {
+                const uint64_t *s = split.at(first + by * i) + tid;
+                const float2 ml = slot_get(s + 8 * DT * AT_THREADS);
+                const float w = __builtin_amdgcn_exp2f(ml.x - ms);
+                L += ml.y * w;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const f4_t s = {o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
-                        *reinterpret_cast<f4u_t *>(dst + 32 * d + 8 * k + 4 * h) = l == 0.0f ? s : s / l;
+                    for (int k = 0; k < 8; k++) {
+                        const float2 x = slot_get(s + (8 * d + k) * AT_THREADS);
+                        sum[d][2 * k] += x.x * w;
+                        sum[d][2 * k + 1] += x.y * w;
                     }
-            } else {
-                float *slot = work + (size_t)(2 * part + (i0 == 0 ? 1 : 0)) * attn_slot(AW_COLS, D);
-#pragma unroll
-                for (int d = 0; d < DT; d++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        *reinterpret_cast<f4_t *>(slot + c * D + 32 * d + 8 * k + 4 * h) =
-                            f4_t{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
-                if (h == 0) {
-                    slot[AW_COLS * D + c] = m;
-                    slot[AW_COLS * (D + 1) + c] = l;
-                }
             }
-        }
-        if (i0 == 0 && !mine) {
-            left_count = (int)(kv_part(W, n, tend - 1) - part) + 1;
-            left_row0 = t.row0;
-            left_c0 = c0;
-            left_ncol = ncol;
-            left_head = t.head;
-        }
+            if (into) keep(into, sum, M, L);
+            else result(sum, L);
+        });
     }
-    if (tid == 0) joins[part] = AtJoin{left_count, left_row0, left_c0, left_ncol, left_head, {0, 0, 0}};
-}
-
-// The tiles that cuts separate: workgroup (w, y) takes columns y JC .. of the
-// tile that part w leaves to those behind it.  A thread holds four dimensions
-// of a column, and CL classes of parts their running maximum and sums.
-template <int COLS, int D, int JC>
-__global__ __launch_bounds__(256) void kv_attn_join_kernel(KvAttn a, const AtJoin *__restrict__ joins)
-{
-    constexpr int LN = D / 4, CL = 256 / (LN * JC), AHEAD = JC == 1 ? 8 : 2;
-    __shared__ float sms[JC][CL], sls[JC][CL];
-    __shared__ __align__(16) f4_t sos[JC][CL][LN];
-    const AtJoin t = joins[blockIdx.x];
-    if ((int)blockIdx.y * JC >= t.ncol || t.count == 0) return;
-    const float *work = reinterpret_cast<const float *>(joins + gridDim.x);
-    // (threads behind the last column or class do its work beside it and store nothing)
-    const int jc = threadIdx.x / (LN * CL) % JC, ln = threadIdx.x % LN;
-    const int cl = threadIdx.x < LN * CL * JC ? threadIdx.x / LN % CL : CL;
-    const int c = min((int)blockIdx.y * JC + jc, t.ncol - 1);
-    float *const sm = sms[jc], *const sl = sls[jc];
-    f4_t(*const so)[LN] = sos[jc];
-    float M = -INFINITY, L = 0.0f;
-    f4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (cl < CL)
-        for (int k0 = cl; k0 < t.count; k0 += AHEAD * CL) {
-            float m[AHEAD], l[AHEAD];
-            f4_t o[AHEAD];
-#pragma unroll
-            for (int u = 0; u < AHEAD; u++) {
-                const int k = min(k0 + u * CL, t.count - 1);
-                const float *s = work + (size_t)(2 * (blockIdx.x + k) + (k == 0)) * attn_slot(COLS, D);
-                m[u] = s[COLS * D + c];
-                l[u] = s[COLS * (D + 1) + c];
-                o[u] = *reinterpret_cast<const f4_t *>(s + c * D + 4 * ln);
-            }
-            float top = M;
-#pragma unroll
-            for (int u = 0; u < AHEAD; u++)
-                if (k0 + u * CL < t.count) top = fmaxf(top, m[u]);
-            const float ms = top == -INFINITY ? 0.0f : top;
-            const float r = __builtin_amdgcn_exp2f(M - ms);
-            sum *= r;
-            L *= r;
-#pragma unroll
-            for (int u = 0; u < AHEAD; u++)
-                if (k0 + u * CL < t.count) {
-                    const float w = __builtin_amdgcn_exp2f(m[u] - ms);
-                    sum += o[u] * w;
-                    L += l[u] * w;
-                }
-            M = top;
-        }
-    if (cl < CL) {
-        so[cl][ln] = sum;
-        if (ln == 0) {
-            sm[cl] = M;
-            sl[cl] = L;
-        }
-    }
-    __syncthreads();
-    if (cl != 0 || (int)blockIdx.y * JC + jc >= t.ncol) return;
-    const int top = min(CL, t.count);
-    M = sm[0];
-    for (int k = 1; k < top; k++) M = fmaxf(M, sm[k]);
-    const float ms = M == -INFINITY ? 0.0f : M;
-    sum = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    L = 0.0f;
-    for (int k = 0; k < top; k++) {
-        const float w = __builtin_amdgcn_exp2f(sm[k] - ms);
-        sum += so[k][ln] * w;
-        L += sl[k] * w;
-    }
-    const int row = t.row0 + (t.c0 + c) / a.group, head = t.head * a.group + (t.c0 + c) % a.group;
-    const f4_t out = L == 0.0f ? sum : sum / L;
-    *reinterpret_cast<f4u_t *>(a.out + ((size_t)row * a.n_heads + head) * D + 4 * ln) = out;
 }
 
 template <class E, int D>
 static void attn_launch_d(qq_ctx *ctx, const qq_kv *kv, const KvBatch &b, const KvAttn &a)
 {
     const size_t shm = at_plan_bytes(b);
-    AtJoin *joins = reinterpret_cast<AtJoin *>(kv->work);
+    uint32_t *work = kv->work;
     // Many rows a sequence: more than two narrow tiles' columns.
     const bool wide = b.row_start && (int64_t)b.n_rows * a.group > (int64_t)2 * AT_COLS * b.n_seqs;
     const int parts = wide ? wide_parts(ctx) : attn_parts(ctx, D);
     prof_begin(ctx, K_KV_ATTN);
     if (wide)
-        QQ_LAUNCH(ctx, (kv_attn_wide_kernel<E, D>), dim3(parts), dim3(AT_THREADS), shm, b, a, joins);
+        QQ_LAUNCH(ctx, (kv_attn_wide_kernel<E, D>), dim3(parts), dim3(AT_THREADS), shm, b, a, work);
     else if (b.row_start)
-        QQ_LAUNCH(ctx, (kv_attn_kernel<E, D, true>), dim3(parts), dim3(AT_THREADS), shm, b, a, joins);
+        QQ_LAUNCH(ctx, (kv_attn_kernel<E, D, true>), dim3(parts), dim3(AT_THREADS), shm, b, a, work);
     else
-        QQ_LAUNCH(ctx, (kv_attn_kernel<E, D, false>), dim3(parts), dim3(AT_THREADS), shm, b, a, joins);
-    prof_begin(ctx, K_KV_JOIN);
-    constexpr int JC = 128 / (D / 4);   // two classes of parts: a wide tile's are few
-    if (wide)
-        QQ_LAUNCH(ctx, (kv_attn_join_kernel<AW_COLS, D, JC>), dim3(parts, (AW_COLS + JC - 1) / JC), dim3(256), 0, a, joins);
-    else
-        QQ_LAUNCH(ctx, (kv_attn_join_kernel<AT_COLS, D, 1>),
-                  dim3(parts, b.row_start ? AT_COLS : std::min(AT_COLS, a.group)), dim3(256), 0, a, joins);
+        QQ_LAUNCH(ctx, (kv_attn_kernel<E, D, false>), dim3(parts), dim3(AT_THREADS), shm, b, a, work);
     prof_end(ctx);
 }
 

@@ -307,11 +307,15 @@ int qq_kv_create(qq_ctx *ctx, void *pool_dev, size_t nbytes, int n_layers, int n
     }
     if (e == hipSuccess) {
         void *v = nullptr;
-        e = hipMalloc(&v, kv_attn_work_bytes(ctx, s));
-        kv->work = static_cast<float *>(v);
+        const size_t n = kv_attn_work_bytes(ctx, s);
+        e = hipMalloc(&v, n);
+        kv->work = static_cast<uint32_t *>(v);
+        if (e == hipSuccess) e = hipMemsetAsync(v, 0, n, ctx->stream);   // its counters start at zero
+        if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
     }
     if (e != hipSuccess) {
         if (kv->own_pool && kv->pool) (void)hipFree(kv->pool);
+        if (kv->work) (void)hipFree(kv->work);
         delete kv;
         return check_hip(ctx, e, "kv_create");
     }

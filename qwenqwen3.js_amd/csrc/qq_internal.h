@@ -133,7 +133,7 @@ struct qq_kv {
     char *pool = nullptr;
     size_t nbytes = 0;
     bool own_pool = false;
-    float *work = nullptr;   // the attention's workspace
+    uint32_t *work = nullptr;   // the attention's workspace
 };
 
 // Layers of one MoE stack (qq_moe_stack_create): borrowed layer handles, their
@@ -225,7 +225,6 @@ enum KernelId {
     K_ROW_INV,
     K_KV_STORE,
     K_KV_ATTN,
-    K_KV_JOIN,
     K_KV_PAGES,
     K_COUNT
 };
