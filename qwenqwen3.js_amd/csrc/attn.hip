@@ -257,6 +257,7 @@ __device__ __forceinline__ float half_sum(float v)
 // Tiles count by sequence, then column tile, the same for every key/value
 // head; heads are the outer order.  A thread weighs T / NT tiles in a row; a
 // step is found by a search over those runs and a walk through one of them.
+// Up to 64 tiles of one row each, every wave has for itself, one a lane.
 struct AtTile {
     int seq, head, t;        // sequence, key/value head, column tile
     int row0, rows, len;     // the sequence's new rows and length
@@ -312,6 +313,9 @@ struct AtWork {
     int per;          // tiles of a run
     int each;         // tiles of a sequence of one row
     uint64_t S;       // steps of one head
+    bool few;         // a tile a lane: its first step and its sequence's length
+    uint32_t lane_start;
+    int lane_len;
 
     __device__ AtWork(const KvBatch &b_, const KvAttn &a_, AtPlan<NT> &p_, int *lds)
         : b(b_), a(a_), p(p_), len(lds), first(lds + b_.n_seqs), row0(lds + 2 * b_.n_seqs + 1),
@@ -360,6 +364,23 @@ struct AtWork {
     {
         const int tid = threadIdx.x;
         int T = b.n_seqs * each;
+        few = !ROWS && T <= WAVE && ((int64_t)b.stride << b.s.page_log) <= 1 << 28;   // steps in 32 bits
+        if (few) {
+            const int g = tid & (WAVE - 1);
+            int seq, t;
+            place(min(g, T - 1), seq, t);
+            lane_len = max(b.len[seq], 0);
+            const uint32_t own = g < T ? span(lane_len, 1, t).n + LEAD : 0;
+            uint32_t inc = own;
+#pragma unroll
+            for (int o = 1; o < WAVE; o <<= 1) {
+                const uint32_t up = __shfl_up(inc, o, WAVE);
+                if (g >= o) inc += up;
+            }
+            lane_start = inc - own;
+            S = (uint32_t)__builtin_amdgcn_readlane((int)inc, WAVE - 1);
+            return S * b.s.n_kv_heads;
+        }
         for (int s = tid; s < b.n_seqs; s += NT) len[s] = max(b.len[s], 0);
         if (ROWS) {
             const int run = (b.n_seqs + NT - 1) / NT, s0 = min(tid * run, b.n_seqs), s1 = min(s0 + run, b.n_seqs);
@@ -401,8 +422,19 @@ struct AtWork {
     __device__ __forceinline__ AtTile find(uint64_t x) const
     {
         AtTile t;
-        t.head = (int)(x / S);
+        t.head = (int)kv_div(x, S);
         const uint64_t base = S * t.head, r = x - base;
+        if (few) {
+            // the last tile that starts at or ahead of r (those behind the last start at S)
+            const int g = 63 - __builtin_clzll(__ballot(lane_start <= (uint32_t)r));
+            place(g, t.seq, t.t);
+            t.len = __builtin_amdgcn_readlane(lane_len, g);
+            t.rows = 1;
+            t.row0 = t.seq;
+            t.span = span(t.len, 1, t.t);
+            t.start = base + (uint32_t)__builtin_amdgcn_readlane((int)lane_start, g);
+            return t;
+        }
         int lo = 0, hi = NT - 1;         // the last run that starts at or ahead of r
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
@@ -825,7 +857,8 @@ __global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBat
 // consecutive units.  Row m = 8 a + 4 h + b of 32 is position 16 (a / 2) + 8 h
 // + 4 (a % 2) + b of 16-bit types, m of fp32: the scores of a lane's half h
 // then are those of whole units of V.
-template <class E, int D>
+// ONE: pages of a stage or more.
+template <class E, int D, bool ONE>
 __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvBatch b, KvAttn a, uint32_t *work)
 {
     typedef AtOps<E> Ops;
@@ -885,20 +918,27 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
         const int tl1 = a.window && tp1 >= 0 ? max(tp1 - a.window + 1, 0) : 0;
 
         // Table entries of the next copies, and the copies (which return which
-        // of the stage's positions, in the rows' order, have a page).  Pages of
-        // a stage or more: one entry, and lanes that differ by a constant.
-        const bool one = ps >= P;
+        // of the stage's positions, in the rows' order, have a page).  With one
+        // page a stage its number is a scalar, and lanes differ by a constant: a
+        // 4096-token prompt 171 us, not 174.  (No load under a branch: it would be
+        // waited for where the branch ends.)
+        typedef const int32_t __attribute__((address_space(4))) *scalar_t;    // read by the scalar unit
+        const scalar_t row = (scalar_t)(uintptr_t)(b.table + (size_t)t.seq * b.stride);
         int ek, ev[NV];
         auto entries = [&](int i) {
             const int base = kv_base(t.span, min(i, i1 - 1), SLOG);
-            ek = kv_entry(b, t.seq, base + kp);   // (no branch: what is loaded under one is waited for at its end)
+            if constexpr (ONE) {
+                ek = row[min(base >> b.s.page_log, b.stride - 1)];
+            } else {
+                ek = kv_entry(b, t.seq, base + kp);
 #pragma unroll
-            for (int k = 0; k < NV; k++) ev[k] = kv_entry(b, t.seq, base + (k * AT_THREADS + tid) / D * U);
+                for (int k = 0; k < NV; k++) ev[k] = kv_entry(b, t.seq, base + (k * AT_THREADS + tid) / D * U);
+            }
         };
         auto copy = [&](int i, int buf) -> uint64_t {
             const int base = kv_base(t.span, i, SLOG);
-            if (one) {
-                const int g = uni(kv_page_of(b, base, ek)), slot = base & (ps - 1);
+            if constexpr (ONE) {
+                const int g = kv_page_of(b, base, ek), slot = base & (ps - 1);
                 const char *page = b.pool + (size_t)max(g, 0) * b.s.page_bytes;
                 const char *kb = page + ((size_t)t.head * (D / U) * ps + slot) * 16;
                 const char *vb = page + vbase + ((size_t)t.head * ps + slot) * (D / U) * 16;
@@ -1169,8 +1209,10 @@ static void attn_launch_d(qq_ctx *ctx, const qq_kv *kv, const KvBatch &b, const 
     const bool wide = b.row_start && (int64_t)b.n_rows * a.group > (int64_t)2 * AT_COLS * b.n_seqs;
     const int parts = wide ? wide_parts(ctx) : attn_parts(ctx, D);
     prof_begin(ctx, K_KV_ATTN);
-    if (wide)
-        QQ_LAUNCH(ctx, (kv_attn_wide_kernel<E, D>), dim3(parts), dim3(AT_THREADS), shm, b, a, work);
+    if (wide && b.s.page_size >= (E::U == 4 ? 32 : 64))
+        QQ_LAUNCH(ctx, (kv_attn_wide_kernel<E, D, true>), dim3(parts), dim3(AT_THREADS), shm, b, a, work);
+    else if (wide)
+        QQ_LAUNCH(ctx, (kv_attn_wide_kernel<E, D, false>), dim3(parts), dim3(AT_THREADS), shm, b, a, work);
     else if (b.row_start)
         QQ_LAUNCH(ctx, (kv_attn_kernel<E, D, true>), dim3(parts), dim3(AT_THREADS), shm, b, a, work);
     else

@@ -53,6 +53,11 @@ __device__ __forceinline__ bool kv_row(const KvBatch &b, int t, int &seq, int &p
         seq = t;
     } else {
         int lo = 0, hi = b.n_seqs - 1;   // the last sequence that starts at or ahead of t
+        if (b.n_seqs <= WAVE) {          // by one load of the wave's (all of its lanes are here, for one t)
+            const int l = threadIdx.x & (WAVE - 1);
+            const uint64_t ahead = __ballot(b.row_start[min(l, hi)] <= t && l <= hi);
+            lo = hi = ahead ? 63 - __builtin_clzll(ahead) : 0;
+        }
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
             if (b.row_start[mid] <= t) lo = mid;
