@@ -301,10 +301,10 @@ int qq_kv_pool_bytes(int n_layers, int n_pages, int page_size, int n_kv_heads, i
                      size_t *nbytes);
 /* A pool over the caller's device memory (pool_dev, 16-byte aligned, nbytes
  * at least qq_kv_pool_bytes; it must outlive the handle, its values are kept)
- * or, with pool_dev NULL, over zeroed memory of its own.  The handle also
- * holds the attention's workspace, of a size that no call changes.  Its calls
- * are made on the context that created it, in the order of that context's
- * stream. */
+ * or, with pool_dev NULL, over zeroed memory of its own.  A context's first
+ * pool also brings the attention's workspace (70 MB, of a size that no call
+ * changes, so captured graphs keep it).  A pool's calls are made on the
+ * context that created it, in the order of that context's stream. */
 int qq_kv_create(qq_ctx *ctx, void *pool_dev, size_t nbytes, int n_layers, int n_pages, int page_size,
                  int n_kv_heads, int head_dim, int type, qq_kv **out);
 int qq_kv_release(qq_ctx *ctx, qq_kv *kv);

@@ -336,6 +336,7 @@ void qq_destroy(qq_ctx *ctx)
     (void)hipStreamSynchronize(ctx->stream);
     if (ctx->scratch) (void)hipFree(ctx->scratch);
     if (ctx->pinned) (void)hipHostFree(ctx->pinned);
+    if (ctx->kv_work) (void)hipFree(ctx->kv_work);
     (void)hipEventDestroy(ctx->ev0);
     (void)hipEventDestroy(ctx->ev1);
     if (ctx->sync_slots) (void)hipFree(ctx->sync_slots);

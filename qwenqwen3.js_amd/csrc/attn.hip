@@ -50,30 +50,35 @@ constexpr int AT_WAVES = 4;      // waves of a workgroup
 constexpr int AT_THREADS = AT_WAVES * WAVE;
 constexpr int AT_LEAD = 4;       // steps that a tile's beginning and end are worth
 constexpr int AT_LEAST = 4;      // steps a part has at least
+constexpr int AT_MAX_PARTS = 4096;
 constexpr int AT_GROUP = 16;     // parts of a tile that one workgroup joins
 // workgroups a CU holds, by registers: a wave keeps two steps of values and one of keys, q's planes and the sums
 __host__ __device__ constexpr int at_per_cu(int dim) { return dim <= 64 ? 3 : 2; }
 
-static int attn_parts(const qq_ctx *ctx, int dim) { return std::min(ctx->num_cus * at_per_cu(dim), 4095); }
+static int attn_parts(const qq_ctx *ctx, int dim) { return std::min(ctx->num_cus * at_per_cu(dim), AT_MAX_PARTS - 1); }
 // The form for many rows: 128 columns, 32 a wave
 constexpr int AW_COLS = 128;
 constexpr int AW_LEAD = 2;
 constexpr int AW_GROUP = 8;
 constexpr int AW_PER_CU = 2;
-static int wide_parts(const qq_ctx *ctx) { return std::min(ctx->num_cus * AW_PER_CU, 4095); }
+static int wide_parts(const qq_ctx *ctx) { return std::min(ctx->num_cus * AW_PER_CU, AT_MAX_PARTS - 1); }
 
-// The workspace: counters of arrived parts, zero between launches (who finds
-// its tile complete clears them), three for every workgroup; then its slots,
+// The workspace, one a context: counters of arrived parts, zero between
+// launches (who finds its tile complete clears them), three for every
+// workgroup; then its slots,
 // in words of two floats: the columns' D sums (two planes of half of every
 // four, or each thread's), then maximum and sum of probabilities of a column,
 // or of each thread's.
 __host__ __device__ constexpr int attn_slot(int cols, int dim) { return cols * (dim / 2 + 2); }
-__host__ __device__ constexpr size_t attn_counters(int parts) { return ((size_t)parts * 3 + 63) / 64 * 64; }
-size_t kv_attn_work_bytes(const qq_ctx *ctx, const KvShape &s)
+constexpr int AT_COUNTERS = 3 * AT_MAX_PARTS;   // their place depends on no launch: no slot may lie where another's counters do
+size_t kv_attn_counter_bytes() { return sizeof(uint32_t) * AT_COUNTERS; }
+size_t kv_attn_work_bytes(const qq_ctx *ctx)
 {
-    const int narrow = attn_parts(ctx, s.head_dim), wide = wide_parts(ctx);
-    return 4 * attn_counters(std::max(narrow, wide)) + 8 * std::max((size_t)narrow * 2 * attn_slot(AT_COLS, s.head_dim),
-                                                                   (size_t)wide * 2 * attn_slot(AW_COLS, s.head_dim));
+    size_t words = 0;
+    for (int dim = 32; dim <= KV_MAX_DIM; dim += 32)
+        words = std::max({words, (size_t)attn_parts(ctx, dim) * 2 * attn_slot(AT_COLS, dim),
+                          (size_t)wide_parts(ctx) * 2 * attn_slot(AW_COLS, dim)});
+    return kv_attn_counter_bytes() + sizeof(uint64_t) * words;
 }
 
 // Two fp32 rounded to fp16 in one register, and what rounding left of either
@@ -483,12 +488,12 @@ __device__ __forceinline__ float2 slot_get(const uint64_t *p)
 struct AtSplit {
     uint32_t *counters;
     uint64_t *slots;
-    uint32_t parts, w0;
+    uint32_t w0;
     int k, count, slot;     // slot: words of one
 
-    __device__ __forceinline__ AtSplit(uint32_t *work, uint32_t grid, int slot_, uint64_t W, uint32_t n, uint32_t part,
+    __device__ __forceinline__ AtSplit(uint32_t *work, int slot_, uint64_t W, uint32_t n, uint32_t part,
                                        uint64_t own, uint64_t tend)
-        : counters(work), slots(reinterpret_cast<uint64_t *>(work + attn_counters(grid))), parts(grid), slot(slot_)
+        : counters(work), slots(reinterpret_cast<uint64_t *>(work + AT_COUNTERS)), slot(slot_)
     {
         w0 = kv_part(W, n, own);
         count = (int)(kv_part(W, n, tend - 1) - w0) + 1;
@@ -522,7 +527,7 @@ struct AtSplit {
         }
         const int g = k / GROUP, first = g * GROUP, size = min(GROUP, count - first);
         // (a workgroup may be the first of one tile and in the middle of another)
-        if (!last(counters + (g == 0 ? parts : 2 * parts) + w0 + first, size, said)) return;
+        if (!last(counters + (g == 0 ? 1 : 2) * AT_MAX_PARTS + w0 + first, size, said)) return;
         join(first, 1, size, at(first));
         if (last(counters + w0, (count + GROUP - 1) / GROUP, said)) join(0, GROUP, (count + GROUP - 1) / GROUP, nullptr);
     }
@@ -773,7 +778,7 @@ __global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBat
         __syncthreads();
         // whole: the result; else this workgroup's part of it
         const bool mine = i0 == 0 && i1 == t.span.n;
-        const AtSplit split(work, gridDim.x, attn_slot(AT_COLS, D), W, n, blockIdx.x, own, tend);
+        const AtSplit split(work, attn_slot(AT_COLS, D), W, n, blockIdx.x, own, tend);
         auto result = [&](int c, int d, const f4_t &sum, float L) {
             const int row = t.row0 + (c0 + c) / grp, head = t.head * grp + (c0 + c) % grp;
             // nothing seen: L = 0 and a sum of zeros
@@ -1170,7 +1175,7 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
             if (c < ncol) result(o, l);
             continue;
         }
-        const AtSplit split(work, gridDim.x, attn_slot(AW_COLS, D), W, n, part, own, tend);
+        const AtSplit split(work, attn_slot(AW_COLS, D), W, n, part, own, tend);
         if (c < ncol) keep(split.at(split.k), o, m, l);
         split.template bring<AW_GROUP>(&said, [&](int first, int by, int num, uint64_t *into) {
             if (c >= ncol) return;
@@ -1201,10 +1206,10 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
 }
 
 template <class E, int D>
-static void attn_launch_d(qq_ctx *ctx, const qq_kv *kv, const KvBatch &b, const KvAttn &a)
+static void attn_launch_d(qq_ctx *ctx, const KvBatch &b, const KvAttn &a)
 {
     const size_t shm = at_plan_bytes(b);
-    uint32_t *work = kv->work;
+    uint32_t *work = ctx->kv_work;
     // Many rows a sequence: more than two narrow tiles' columns.
     const bool wide = b.row_start && (int64_t)b.n_rows * a.group > (int64_t)2 * AT_COLS * b.n_seqs;
     const int parts = wide ? wide_parts(ctx) : attn_parts(ctx, D);
@@ -1221,21 +1226,21 @@ static void attn_launch_d(qq_ctx *ctx, const qq_kv *kv, const KvBatch &b, const 
 }
 
 template <class E>
-static void attn_launch(qq_ctx *ctx, const qq_kv *kv, const KvBatch &b, const KvAttn &a)
+static void attn_launch(qq_ctx *ctx, const KvBatch &b, const KvAttn &a)
 {
     switch (b.s.head_dim) {
-    case 32: attn_launch_d<E, 32>(ctx, kv, b, a); break;
-    case 64: attn_launch_d<E, 64>(ctx, kv, b, a); break;
-    case 96: attn_launch_d<E, 96>(ctx, kv, b, a); break;
-    default: attn_launch_d<E, 128>(ctx, kv, b, a); break;
+    case 32: attn_launch_d<E, 32>(ctx, b, a); break;
+    case 64: attn_launch_d<E, 64>(ctx, b, a); break;
+    case 96: attn_launch_d<E, 96>(ctx, b, a); break;
+    default: attn_launch_d<E, 128>(ctx, b, a); break;
     }
 }
 
-int launch_kv_attn(qq_ctx *ctx, const qq_kv *kv, const KvBatch &b, const KvAttn &a)
+int launch_kv_attn(qq_ctx *ctx, const KvBatch &b, const KvAttn &a)
 {
-    if (b.s.type == QQ_TYPE_F32) attn_launch<KvF32>(ctx, kv, b, a);
-    else if (b.s.type == QQ_TYPE_F16) attn_launch<KvF16>(ctx, kv, b, a);
-    else attn_launch<KvBf16>(ctx, kv, b, a);
+    if (b.s.type == QQ_TYPE_F32) attn_launch<KvF32>(ctx, b, a);
+    else if (b.s.type == QQ_TYPE_F16) attn_launch<KvF16>(ctx, b, a);
+    else attn_launch<KvBf16>(ctx, b, a);
     QQ_HIP(ctx, hipGetLastError());
     return QQ_OK;
 }

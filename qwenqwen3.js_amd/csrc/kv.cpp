@@ -305,17 +305,16 @@ int qq_kv_create(qq_ctx *ctx, void *pool_dev, size_t nbytes, int n_layers, int n
         if (e == hipSuccess) e = hipMemsetAsync(v, 0, need, ctx->stream);
         if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
     }
-    if (e == hipSuccess) {
+    if (e == hipSuccess && !ctx->kv_work) {
         void *v = nullptr;
-        const size_t n = kv_attn_work_bytes(ctx, s);
-        e = hipMalloc(&v, n);
-        kv->work = static_cast<uint32_t *>(v);
-        if (e == hipSuccess) e = hipMemsetAsync(v, 0, n, ctx->stream);   // its counters start at zero
+        e = hipMalloc(&v, kv_attn_work_bytes(ctx));
+        if (e == hipSuccess) e = hipMemsetAsync(v, 0, kv_attn_counter_bytes(), ctx->stream);
         if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+        if (e == hipSuccess) ctx->kv_work = static_cast<uint32_t *>(v);
+        else if (v) (void)hipFree(v);
     }
     if (e != hipSuccess) {
         if (kv->own_pool && kv->pool) (void)hipFree(kv->pool);
-        if (kv->work) (void)hipFree(kv->work);
         delete kv;
         return check_hip(ctx, e, "kv_create");
     }
@@ -339,7 +338,6 @@ int qq_kv_release(qq_ctx *ctx, qq_kv *kv)
     QQ_HIP(ctx, hipSetDevice(ctx->device));
     QQ_HIP(ctx, hipStreamSynchronize(ctx->stream));
     if (kv->own_pool) (void)hipFree(kv->pool);
-    (void)hipFree(kv->work);
     delete kv;
     return QQ_OK;
 }
@@ -456,7 +454,7 @@ int qq_kv_attn_dev(qq_ctx *ctx, qq_kv *kv, int layer, const qq_kv_batch *batch, 
     a.scale = scale;
     a.window = window;
     a.sinks = window ? sinks : 0;
-    return launch_kv_attn(ctx, kv, device_batch(kv, layer, batch), a);
+    return launch_kv_attn(ctx, device_batch(kv, layer, batch), a);
 }
 
 int qq_kv_copy_pages_dev(qq_ctx *ctx, qq_kv *kv, const int32_t *pairs_dev, int n)

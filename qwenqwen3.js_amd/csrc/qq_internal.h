@@ -133,7 +133,6 @@ struct qq_kv {
     char *pool = nullptr;
     size_t nbytes = 0;
     bool own_pool = false;
-    uint32_t *work = nullptr;   // the attention's workspace
 };
 
 // Layers of one MoE stack (qq_moe_stack_create): borrowed layer handles, their
@@ -179,6 +178,7 @@ struct qq_ctx {
     uint64_t *sync_hloc, *sync_hdev, *sync_part, *sync_arrive, *sync_hx, *sync_rp, *sync_ri;
     uint32_t *sync_seg;   // SEG_CTR_WORDS stream-kernel segment counters and generations
     uint64_t *seg_part;   // num_cus x SEG_PART_WORDS partial sums
+    uint32_t *kv_work;    // the paged attention's workspace (attn.hip), from the first qq_kv_create on
     float *rows_part;     // num_cus x 32 KiB: partial sums of split Q8_0 row products (rows.hip)
     // device-side waits that timed out on this context so far (counted when
     // the error word is read); device-resident state built across calls (an
@@ -436,8 +436,11 @@ struct KvAttn {
     double scale;
 };
 int launch_kv_store(qq_ctx *ctx, const KvBatch &b, const KvStore &st);
-size_t kv_attn_work_bytes(const qq_ctx *ctx, const KvShape &s);
-int launch_kv_attn(qq_ctx *ctx, const qq_kv *kv, const KvBatch &b, const KvAttn &a);
+// The attention's workspace: of one size for every shape, its first bytes
+// (counters) zero between launches.
+size_t kv_attn_work_bytes(const qq_ctx *ctx);
+size_t kv_attn_counter_bytes();
+int launch_kv_attn(qq_ctx *ctx, const KvBatch &b, const KvAttn &a);
 int launch_kv_copy(qq_ctx *ctx, const KvShape &s, char *pool, const int32_t *pairs, int n);
 int launch_kv_remap(qq_ctx *ctx, int32_t *table, int n, const int32_t *map, int n_map);
 int launch_moe_grouped(qq_ctx *ctx, const qq_moe *m, const float *x, float *hidden, int T,

@@ -597,6 +597,24 @@ def test_graphs_follow_lengths_and_tables():
         kv.release()
 
 
+def test_calls_of_every_form_in_turn():
+    """Calls that split their work differently share the context's workspace: whatever ran before, the next is right."""
+    ctx = gpu_context()
+    forms = [Batch([9000], None, 4, 1, 64, F16, 64, fill=0.5), Batch([2000], [300], 4, 1, 64, F16, 64, fill=0.5, seed=1),
+             Batch([9000, 30], None, 8, 2, 128, BF16, 32, fill=0.5), Batch([5000], [40], 8, 1, 128, F32, 64, fill=0.5),
+             Batch([9000, 100, 7], [3, 1, 2], 4, 1, 32, F16, 16, fill=0.5), Batch([1500], [1500], 2, 2, 96, BF16, 16, fill=0.5)]
+    kvs = [b.kv(ctx) for b in forms]
+    refs = [b.ref(0.1) for b in forms]
+    try:
+        for i in (0, 1, 0, 2, 3, 0, 4, 5, 2, 4, 1, 0, 5, 3, 2):
+            forms[i].d_out.fill_(77.0)
+            _torch().cuda.synchronize()
+            _check(forms[i].attn(ctx, kvs[i], 0.1), *refs[i], i)
+    finally:
+        for kv in kvs:
+            kv.release()
+
+
 def test_on_the_callers_stream():
     torch = _torch()
     with qq_hip.Context(0) as ctx:
