@@ -389,17 +389,19 @@ struct AtWork {
         for (int s = tid; s < b.n_seqs; s += NT) len[s] = max(b.len[s], 0);
         if (ROWS) {
             const int run = (b.n_seqs + NT - 1) / NT, s0 = min(tid * run, b.n_seqs), s1 = min(s0 + run, b.n_seqs);
-            int sum = 0;
+            uint64_t sum = 0, all;
             for (int s = s0; s < s1; s++) {
                 int r0, r1;
                 kv_rows(b, s, r0, r1);
                 row0[s] = r0;
                 rows[s] = r1 - r0;
-                first[s] = sum;
+                first[s] = (int)sum;
                 sum += kv_tiles(r1 - r0, a.group, COLS);
             }
-            const int off = at_scan<int, NT>(sum, T, p.red);
-            for (int s = s0; s < s1; s++) first[s] += off;
+            const uint64_t off = at_scan<uint64_t, NT>(sum, all, p.red);
+            for (int s = s0; s < s1; s++) first[s] += (int)off;
+            // more tiles than rows make: row_start falls, and the call does nothing
+            T = all <= ((uint64_t)b.n_rows * a.group + COLS - 1) / COLS + b.n_seqs ? (int)all : 0;
             if (tid == 0) first[b.n_seqs] = T;
         }
         __syncthreads();

@@ -183,6 +183,48 @@ def test_many_sequences():
     _run([int(x) for x in rng.integers(0, 40, 4096)], None, (2, 1, 32), "f16", 16)
 
 
+@pytest.mark.parametrize("heads,news", [((2, 1, 128), 2), ((16, 1, 128), 3), ((1, 1, 32), 1)], ids=str)
+def test_many_sequences_with_rows(heads, news):
+    """As many sequences as a call takes, several rows each (either form), with row_start."""
+    torch, ctx = _torch(), gpu_context()
+    n, ps, (nq, nkv, dim) = 4096, 16, heads
+    rng = np.random.default_rng(6)
+    lens = rng.integers(news, 2 * ps, n)
+    kv = ctx.kv_pool(1, 2 * n, ps, nkv, dim, F32)
+    try:
+        table = _up(rng.permutation(2 * n).reshape(n, 2).astype(np.int32))
+        every = np.concatenate([[0], np.cumsum(lens)])
+        k, v = (rng.standard_normal((int(every[-1]), nkv, dim)).astype(np.float32) for _ in range(2))
+        q = rng.standard_normal((n * news, nq, dim)).astype(np.float32)
+        dk, dv, dq, dl, de = _up(k), _up(v), _up(q), _up(lens.astype(np.int32)), _up(every.astype(np.int32))
+        ds = _up((np.arange(n + 1) * news).astype(np.int32))
+        out = torch.full((n * news, nq, dim), 77.0, device="cuda")
+        torch.cuda.synchronize()
+        kv.store_dev(0, qq_hip.KvBatch(n, table.data_ptr(), 2, dl.data_ptr(), de.data_ptr(), int(every[-1])), dk.data_ptr(),
+                     dv.data_ptr())
+        kv.attn_dev(0, qq_hip.KvBatch(n, table.data_ptr(), 2, dl.data_ptr(), ds.data_ptr(), n * news), dq.data_ptr(), nq,
+                    out.data_ptr(), 0.1)
+        ctx.synchronize()
+        got = out.cpu().numpy()
+        assert np.isfinite(got).all() and (got != 77.0).all()
+        for b in list(range(0, n, 97)) + [n - 1]:
+            r = slice(b * news, (b + 1) * news)
+            ref, bound = attention(q[r], k[every[b]:every[b + 1]], v[every[b]:every[b + 1]], lens[b] - news + np.arange(news),
+                                   0.1, 0, 0)
+            _check(got[r], ref, bound, b)
+        # row_start that falls again and again: nothing is written outside the rows, and the next call is right
+        bad = _up(np.where(np.arange(n + 1) % 2, n * news, 0).astype(np.int32))
+        torch.cuda.synchronize()
+        kv.attn_dev(0, qq_hip.KvBatch(n, table.data_ptr(), 2, dl.data_ptr(), bad.data_ptr(), n * news), dq.data_ptr(), nq,
+                    out.data_ptr(), 0.1)
+        kv.attn_dev(0, qq_hip.KvBatch(n, table.data_ptr(), 2, dl.data_ptr(), ds.data_ptr(), n * news), dq.data_ptr(), nq,
+                    out.data_ptr(), 0.1)
+        ctx.synchronize()
+        assert (out.cpu().numpy() == got).all()
+    finally:
+        kv.release()
+
+
 def test_wide_scores():
     """Scores of some hundreds: all the weight on few positions, exponentials that vanish elsewhere."""
     for typ in sorted(NAMES):
