@@ -809,10 +809,13 @@ __global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBat
         }
         if (!mine)
             split.template bring<AT_GROUP>(&said, [&](int first, int by, int num, uint64_t *into) {
-                for (int e0 = 0; e0 < ncol * (D / 4); e0 += AT_THREADS) {
-                    // (threads behind the last element do its work and store nothing)
-                    const int e = min(e0 + tid, ncol * (D / 4) - 1), c = e / (D / 4), d = e % (D / 4) * 4;
-                    constexpr int AHEAD = 8;
+                // Whole columns a pass: a pass may leave the joined maximum and
+                // sum of its columns where the parts' were.
+                constexpr int PER = AT_THREADS / (D / 4), AHEAD = 8;
+                for (int cp = 0; cp < ncol; cp += PER) {
+                    // (threads behind the last column do its work and store nothing)
+                    const bool live = tid < PER * (D / 4) && cp + tid / (D / 4) < ncol;
+                    const int c = min(cp + min(tid / (D / 4), PER - 1), ncol - 1), d = tid % (D / 4) * 4;
                     float M = -INFINITY, L = 0.0f;
                     f4_t sum = {0.0f, 0.0f, 0.0f, 0.0f};
                     for (int k = 0; k < num; k += AHEAD) {
@@ -843,7 +846,7 @@ __global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBat
                         M = top;
                     }
                     __syncthreads();    // `into` is one of these slots
-                    if (e0 + tid >= ncol * (D / 4)) continue;
+                    if (!live) continue;
                     if (into) keep(into, c, d, sum, M, L);
                     else result(c, d, sum, L);
                 }

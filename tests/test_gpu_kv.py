@@ -178,6 +178,14 @@ def test_few_rows_each(typ):
     _run([100, 33, 1000, 6, 64, 17], [4, 2, 6, 6, 3, 4], (8, 1, 128), typ, 32)
 
 
+@pytest.mark.parametrize("typ", sorted(NAMES))
+@pytest.mark.parametrize("heads", [(24, 1, 96), (11, 1, 96), (16, 1, 128), (13, 1, 64), (16, 1, 32)], ids=str)
+@pytest.mark.parametrize("news", [None, [2, 1]], ids=str)
+def test_joined_in_groups(news, heads, typ):
+    # one tile in more parts than a workgroup joins, its columns in more than one pass
+    _run([9000, 30], news, heads, typ, 64)
+
+
 def test_many_sequences():
     rng = np.random.default_rng(5)
     _run([int(x) for x in rng.integers(0, 40, 4096)], None, (2, 1, 32), "f16", 16)
