@@ -4,7 +4,7 @@
  * Plain C: opaque handles, host or device pointers, sizes, int status codes.
  * Every entry point returns QQ_OK (0) or a negative QQ_E* code; the message of
  * the last failure on a context is qq_last_error(ctx) (qq_last_error(NULL)
- * reports a failed qq_init).  A binding turns a non-zero status into an
+ * reports a failed qq_init, and what fails without a context).  A binding turns a non-zero status into an
  * exception, as the reference does with `throw new Error(...)`
  * (src/tensor.js:494).
  *
@@ -323,7 +323,7 @@ int qq_kv_pool(const qq_kv *kv, void **pool_dev, size_t *nbytes);
 #define QQ_KV_MAX_SEQS 4096
 typedef struct qq_kv_batch {
     int n_seqs;                    /* at most QQ_KV_MAX_SEQS                  */
-    int n_rows;                    /* rows of q, k, v and out                 */
+    int n_rows;                    /* rows of q, k, v and out, below 2^24     */
     const int32_t *table_dev;      /* [n_seqs][table_stride] page numbers     */
     int table_stride;              /* table_stride * page_size <= 2^30        */
     const int32_t *len_dev;        /* [n_seqs]                                */
@@ -355,8 +355,10 @@ int qq_kv_store_dev(qq_ctx *ctx, qq_kv *kv, int layer, const qq_kv_batch *batch,
  *   q, out [n_rows][n_heads][head_dim] fp32; out must not overlap q
  * q enters its products exactly with a BF16 or F32 pool and to 22 bits beside
  * each head's largest with an F16 one, as the probabilities do; sums are fp32.
- * A visible key or value that is not finite makes its rows' heads NaN or
- * infinite; invisible ones have no effect.  Rows may be many (prompt chunks)
+ * A visible value that is not finite makes its rows' heads NaN or infinite, and
+ * so does a key whose score is not finite, but for a score of -infinity: it
+ * weighs nothing, and a row with no other gives zeros.  Invisible ones have no
+ * effect.  scale times log2 e is finite in fp32.  Rows may be many (prompt chunks)
  * or one a sequence (decode); the work is split over the context's length
  * where rows are few, by the lengths in device memory.  Device pointers;
  * enqueued, not waited for. */
@@ -364,7 +366,7 @@ int qq_kv_attn_dev(qq_ctx *ctx, qq_kv *kv, int layer, const qq_kv_batch *batch, 
                    int n_heads, double scale, int window, int sinks, float *out_dev);
 
 /* pool[pairs[i][1]] = pool[pairs[i][0]], K and V of every layer, for n pairs of
- * page numbers (int32 [n][2], device memory).  A pair with a number that is
+ * page numbers (int32 [n][2], device memory; n below 2^24).  A pair with a number that is
  * no page of the pool is skipped.  No page may be the destination of two
  * pairs, or the destination of one and the source of another.  Enqueued. */
 int qq_kv_copy_pages_dev(qq_ctx *ctx, qq_kv *kv, const int32_t *pairs_dev, int n);
@@ -377,6 +379,7 @@ int qq_kv_remap_dev(qq_ctx *ctx, int32_t *table_dev, int n, const int32_t *map_d
  * and counts their users; the caller uploads the tables and runs the copies
  * it is told to.  Not for use by two threads at once. */
 typedef struct qq_pages qq_pages;
+/* n_pages at most 2^24, as a pool has. */
 int qq_pages_create(int n_pages, int page_size, qq_pages **out);
 int qq_pages_release(qq_pages *p);
 /* An empty sequence; *seq is its number from then on. */
@@ -423,8 +426,8 @@ int qq_profile_kernel_count(void);
 /* ---- graphs ------------------------------------------------------------ */
 
 /* Record the device-pointer calls (qq_moe_forward_dev, qq_q8_0_matvec_dev,
- * qq_rmsnorm_dev) made between qq_capture_begin and qq_capture_end on the
- * context's stream into a HIP graph, and replay it with qq_graph_launch
+ * qq_rmsnorm_dev, qq_kv_*_dev) made between qq_capture_begin and qq_capture_end
+ * on the context's stream into a HIP graph, and replay it with qq_graph_launch
  * (enqueued, not waited for).  A replay runs the same kernels on the same
  * pointers; every decode call draws a fresh router epoch on the device, so
  * replays are independent.  While a capture is open, entry points that copy

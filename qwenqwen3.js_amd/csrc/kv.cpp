@@ -73,7 +73,7 @@ int qq_pages_create(int n_pages, int page_size, qq_pages **out)
 {
     if (!out) return pages_error("qq_pages_create: out is NULL");
     *out = nullptr;
-    if (n_pages < 1 || page_size < 1) return set_error(nullptr, "qq_pages_create: %d pages of %d", n_pages, page_size);
+    if (n_pages < 1 || n_pages > 1 << 24 || page_size < 1) return set_error(nullptr, "qq_pages_create: %d pages of %d", n_pages, page_size);
     qq_pages *p = new (std::nothrow) qq_pages();
     if (!p) return no_memory();
     try {
@@ -263,7 +263,7 @@ static int pool_shape(qq_ctx *ctx, int n_layers, int n_pages, int page_size, int
     s->n_kv_heads = n_kv_heads;
     s->head_dim = head_dim;
     s->type = type;
-    // at most 2^24 bytes a page, 2^36 pages: no overflow
+    // at most 2^26 bytes a page, 2^36 pages: no overflow
     s->page_bytes = (size_t)2 * n_kv_heads * page_size * head_dim * (type == QQ_TYPE_F32 ? 4 : 2);
     return QQ_OK;
 }
@@ -360,7 +360,8 @@ static int batch_check(qq_ctx *ctx, const qq_kv *kv, int layer, const qq_kv_batc
     if (!b) return set_error(ctx, "%s: NULL batch", what);
     if (b->n_seqs < 0 || b->n_seqs > QQ_KV_MAX_SEQS)
         return set_error(ctx, "%s: %d sequences (at most %d)", what, b->n_seqs, QQ_KV_MAX_SEQS);
-    if (b->n_rows < 0 || b->n_rows > 1 << 24) return set_error(ctx, "%s: %d rows", what, b->n_rows);
+    // (a launch's first dimension: below 2^32 threads, 256 a row)
+    if (b->n_rows < 0 || b->n_rows >= 1 << 24) return set_error(ctx, "%s: %d rows", what, b->n_rows);
     if (b->n_seqs == 0 || b->n_rows == 0) return QQ_OK;
     if (!b->table_dev || !b->len_dev) return set_error(ctx, "%s: NULL table or lengths", what);
     if (b->table_stride < 1 || (long long)b->table_stride * kv->s.page_size > 1 << 30)
@@ -434,7 +435,8 @@ int qq_kv_attn_dev(qq_ctx *ctx, qq_kv *kv, int layer, const qq_kv_batch *batch, 
 {
     if (int rc = batch_check(ctx, kv, layer, batch, "kv_attn")) return rc;
     if (int rc = heads_check(ctx, kv, n_heads, "kv_attn")) return rc;
-    if (!std::isfinite(scale)) return set_error(ctx, "kv_attn: scale %g", scale);
+    // (the kernels take powers of two, in fp32)
+    if (!std::isfinite((float)(scale * 1.4426950408889634))) return set_error(ctx, "kv_attn: scale %g", scale);
     if (window < 0 || sinks < 0) return set_error(ctx, "kv_attn: window %d, sinks %d", window, sinks);
     if (batch->n_seqs == 0 || batch->n_rows == 0) return QQ_OK;
     if (!q_dev || !out_dev) return set_error(ctx, "kv_attn: NULL buffer");
@@ -460,7 +462,7 @@ int qq_kv_attn_dev(qq_ctx *ctx, qq_kv *kv, int layer, const qq_kv_batch *batch, 
 int qq_kv_copy_pages_dev(qq_ctx *ctx, qq_kv *kv, const int32_t *pairs_dev, int n)
 {
     if (int rc = kv_check(ctx, kv, "kv_copy_pages")) return rc;
-    if (n < 0 || n > 1 << 24) return set_error(ctx, "kv_copy_pages: %d pairs", n);
+    if (n < 0 || n >= 1 << 24) return set_error(ctx, "kv_copy_pages: %d pairs", n);
     if (n == 0) return QQ_OK;
     if (!pairs_dev) return set_error(ctx, "kv_copy_pages: NULL buffer");
     QQ_HIP(ctx, hipSetDevice(ctx->device));

@@ -192,7 +192,7 @@ __global__ __launch_bounds__(256) void kv_copy_kernel(char *pool, size_t page_by
 
 int launch_kv_copy(qq_ctx *ctx, const KvShape &s, char *pool, const int32_t *pairs, int n)
 {
-    const unsigned pieces = (unsigned)((s.page_bytes + KV_PIECE - 1) / KV_PIECE);   // at most 2^10
+    const unsigned pieces = (unsigned)((s.page_bytes + KV_PIECE - 1) / KV_PIECE);   // at most 2^12
     prof_begin(ctx, K_KV_PAGES);
     QQ_LAUNCH(ctx, kv_copy_kernel, dim3(n, s.n_layers, pieces), dim3(256), 0, pool, s.page_bytes, s.n_pages, pairs);
     prof_end(ctx);

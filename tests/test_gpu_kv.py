@@ -746,6 +746,54 @@ def test_refusals():
         kv.release()
 
 
+def test_refusals_of_what_does_not_fit():
+    torch, ctx = _torch(), gpu_context()
+    b = Batch([40, 20], [1, 1], 8, 2, 64, F16, 16)
+    kv = b.kv(ctx)
+    q, o = b.d_q.data_ptr(), b.d_out.data_ptr()
+    try:
+        many = b.batch(n_rows=1 << 24)       # 2^32 threads
+        for call in (lambda: kv.store_dev(0, many, q, q), lambda: kv.attn_dev(0, many, q, 8, o, 0.1),
+                     lambda: kv.copy_pages_dev(q, 1 << 24), lambda: kv.attn_dev(0, b.batch(), q, 8, o, 3e38),
+                     lambda: kv.attn_dev(0, b.batch(), q, 8, o, -1e39)):
+            with pytest.raises(qq_hip.QQError, match="rows|pairs|scale"):
+                call()
+        ref, bound = b.ref(0.125)
+        _check(b.attn(ctx, kv, 0.125), ref, bound)
+    finally:
+        kv.release()
+
+
+def test_scores_of_minus_infinity():
+    """A key whose score is -infinity weighs nothing; a row that sees no other gives zeros."""
+    ctx = gpu_context()
+    for news in (None, [2], [20]):
+        b = Batch([20], news, 4, 1, 64, F32, 16)
+        b.q[:] = np.abs(b.q) + 0.5
+        b.d_q.copy_(_up(b.q))
+        kept = [p for p in range(20) if p % 3]
+        for p in range(20):
+            if p % 3 == 0:
+                k = b.k[0][p].copy()
+                k[0, 7] = -np.inf
+                b.pool.put(0, b.table[0, p // 16], p % 16, k, b.v[0][p])
+        b.d_pool.copy_(_up(b.pool.raw))
+        _torch().cuda.synchronize()
+        kv = b.kv(ctx)
+        try:
+            got = b.attn(ctx, kv, 0.125)
+        finally:
+            kv.release()
+        pos = 20 - b.n + np.arange(b.n)
+        for r in range(b.n):
+            at = [p for p in kept if p <= pos[r]]
+            if not at:
+                assert (got[r] == 0.0).all()
+                continue
+            ref, bound = attention(b.q[r:r + 1], b.k[0][at], b.v[0][at], np.array([len(at) - 1]), 0.125, 0, 0)
+            _check(got[r:r + 1], ref, bound, (news, r))
+
+
 # ---------------------------------------------------------------- together
 
 def test_serving_run():

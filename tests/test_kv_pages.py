@@ -143,6 +143,12 @@ def test_refusals():
     p.release()
 
 
+def test_more_pages_than_a_pool_has():
+    L, h = qq_hip.load(), ctypes.c_void_p()
+    assert L.qq_pages_create((1 << 24) + 1, 16, ctypes.byref(h)) == -1 and not h.value
+    assert b"pages" in L.qq_last_error(None)
+
+
 def test_pool_bytes():
     L, n = qq_hip.load(), ctypes.c_size_t()
     assert L.qq_kv_pool_bytes(6, 100, 64, 8, 64, qq_hip.TYPE_F16, ctypes.byref(n)) == 0
