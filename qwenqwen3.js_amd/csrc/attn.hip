@@ -52,10 +52,13 @@ constexpr int AT_LEAD = 4;       // steps that a tile's beginning and end are wo
 constexpr int AT_LEAST = 4;      // steps a part has at least
 constexpr int AT_MAX_PARTS = 4096;
 constexpr int AT_GROUP = 16;     // parts of a tile that one workgroup joins
-// workgroups a CU holds, by registers: a wave keeps two steps of values and one of keys, q's planes and the sums
-__host__ __device__ constexpr int at_per_cu(int dim) { return dim <= 64 ? 3 : 2; }
+// Workgroups of a CU.  Registers allow no more with heads of 128 (a wave keeps
+// two steps of values and one of keys, q's planes and the sums); smaller heads
+// fit three, but larger parts are worth more (heads of 64, 64 sequences of 1024
+// and of 4096 positions 25 and 86 us, with three 33 and 92).
+constexpr int AT_PER_CU = 2;
 
-static int attn_parts(const qq_ctx *ctx, int dim) { return std::min(ctx->num_cus * at_per_cu(dim), AT_MAX_PARTS - 1); }
+static int attn_parts(const qq_ctx *ctx) { return std::min(ctx->num_cus * AT_PER_CU, AT_MAX_PARTS - 1); }
 // The form for many rows: 128 columns, 32 a wave
 constexpr int AW_COLS = 128;
 constexpr int AW_LEAD = 2;
@@ -76,7 +79,7 @@ size_t kv_attn_work_bytes(const qq_ctx *ctx)
 {
     size_t words = 0;
     for (int dim = 32; dim <= KV_MAX_DIM; dim += 32)
-        words = std::max({words, (size_t)attn_parts(ctx, dim) * 2 * attn_slot(AT_COLS, dim),
+        words = std::max({words, (size_t)attn_parts(ctx) * 2 * attn_slot(AT_COLS, dim),
                           (size_t)wide_parts(ctx) * 2 * attn_slot(AW_COLS, dim)});
     return kv_attn_counter_bytes() + sizeof(uint64_t) * words;
 }
@@ -538,7 +541,7 @@ struct AtSplit {
 
 // ROWS: a tile's columns may be several rows, that see different positions.
 template <class E, int D, bool ROWS>
-__global__ __launch_bounds__(AT_THREADS, at_per_cu(D)) void kv_attn_kernel(KvBatch b, KvAttn a, uint32_t *work)
+__global__ __launch_bounds__(AT_THREADS, AT_PER_CU) void kv_attn_kernel(KvBatch b, KvAttn a, uint32_t *work)
 {
     typedef AtOps<E> Ops;
     constexpr int U = E::U, TK = U / 4, DS = D / (4 * U), DT = D / 16;
@@ -1036,7 +1039,7 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
                     const bool sees = page & (p <= tp1) & ((p >= ql) | (p < sinks));
                     const bool bad = ((x >> sh & EXP) == EXP) & (tp0 != tp1);
                     odd |= sees & bad;
-                    x = !sees | bad ? x & (U == 4 ? 0u : 0xffff0000u >> sh) : x;
+                    x = (!sees | bad) ? x & (U == 4 ? 0u : 0xffff0000u >> sh) : x;
                 }
                 v = make_uint4(w[0], w[1], w[2], w[3]);
             }
@@ -1158,53 +1161,79 @@ __global__ __launch_bounds__(AT_THREADS, AW_PER_CU) void kv_attn_wide_kernel(KvB
         // ---- results, or this workgroup's part of them ----
         l = half_sum(l);
         const int c = wave * 32 + col;      // this lane's column, dimensions 32 d + 8 k + 4 h ..
-        auto result = [&](const f16_t (&v)[DT], float L) {
-            float *dst = a.out + ((size_t)(t.row0 + cr) * nh + t.head * grp + cc % grp) * D;
+        auto result = [&](int d, const auto &v, float L) {
+            float *dst = a.out + ((size_t)(t.row0 + cr) * nh + t.head * grp + cc % grp) * D + 32 * d;
 #pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const f4_t x = {v[d][4 * k], v[d][4 * k + 1], v[d][4 * k + 2], v[d][4 * k + 3]};
-                    *reinterpret_cast<f4u_t *>(dst + 32 * d + 8 * k + 4 * h) = L == 0.0f ? x : x / L;
-                }
-        };
-        auto keep = [&](uint64_t *slot, const f16_t (&v)[DT], float M, float L) {
-#pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int k = 0; k < 8; k++) slot_put(slot + (8 * d + k) * AT_THREADS + tid, v[d][2 * k], v[d][2 * k + 1]);
-            slot_put(slot + 8 * DT * AT_THREADS + tid, M, L);
+            for (int k = 0; k < 4; k++) {
+                const f4_t x = {v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]};
+                *reinterpret_cast<f4u_t *>(dst + 8 * k + 4 * h) = L == 0.0f ? x : x / L;
+            }
         };
         if (i0 == 0 && i1 == t.span.n) {
-            if (c < ncol) result(o, l);
+            if (c < ncol)
+#pragma unroll
+                for (int d = 0; d < DT; d++) result(d, o[d], l);
             continue;
         }
         const AtSplit split(work, attn_slot(AW_COLS, D), W, n, part, own, tend);
-        if (c < ncol) keep(split.at(split.k), o, m, l);
+        if (c < ncol) {
+            uint64_t *slot = split.at(split.k) + tid;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int k = 0; k < 8; k++) slot_put(slot + (8 * d + k) * AT_THREADS, o[d][2 * k], o[d][2 * k + 1]);
+            slot_put(slot + 8 * DT * AT_THREADS, m, l);
+        }
         split.template bring<AW_GROUP>(&said, [&](int first, int by, int num, uint64_t *into) {
             if (c >= ncol) return;
+            // A thread reads and leaves its own words alone, 16 dimensions at
+            // a time, so many parts' in flight at once.
+            constexpr int AHEAD = 4;
             float M = -INFINITY, L = 0.0f;
-            f16_t sum[DT];
+#pragma unroll 1
+            for (int d = 0; d < DT; d++) {
+                M = -INFINITY;
+                L = 0.0f;
+                float sum[16] = {};
+#pragma unroll 1
+                for (int i = 0; i < num; i += AHEAD) {
+                    float2 ml[AHEAD], v[AHEAD][8];
 #pragma unroll
-            for (int d = 0; d < DT; d++) sum[d] = f16_t{};
-            for (int i = 0; i < num; i++) M = fmaxf(M, slot_get(split.at(first + by * i) + 8 * DT * AT_THREADS + tid).x);
-            const float ms = M == -INFINITY ? 0.0f : M;
-            for (int i = 0; i < num; i++) {
-                const uint64_t *s = split.at(first + by * i) + tid;
-                const float2 ml = slot_get(s + 8 * DT * AT_THREADS);
-                const float w = __builtin_amdgcn_exp2f(ml.x - ms);
-                L += ml.y * w;
+                    for (int u = 0; u < AHEAD; u++) {
+                        const uint64_t *s =    // (a scalar: lanes differ by tid)
+                            reinterpret_cast<const uint64_t *>(uni64((uintptr_t)split.at(first + by * min(i + u, num - 1))));
+                        ml[u] = slot_get(s + 8 * DT * AT_THREADS + tid);
 #pragma unroll
-                for (int d = 0; d < DT; d++)
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        const float2 x = slot_get(s + (8 * d + k) * AT_THREADS);
-                        sum[d][2 * k] += x.x * w;
-                        sum[d][2 * k + 1] += x.y * w;
+                        for (int k = 0; k < 8; k++) v[u][k] = slot_get(s + (8 * d + k) * AT_THREADS + tid);
                     }
+                    float top = M;
+#pragma unroll
+                    for (int u = 0; u < AHEAD; u++) top = fmaxf(top, ml[u].x);
+                    const float ts = top == -INFINITY ? 0.0f : top, r = __builtin_amdgcn_exp2f(M - ts);
+                    M = top;
+                    L *= r;
+#pragma unroll
+                    for (int k = 0; k < 16; k++) sum[k] *= r;
+#pragma unroll
+                    for (int u = 0; u < AHEAD; u++)
+                        if (i + u < num) {
+                            const float w = __builtin_amdgcn_exp2f(ml[u].x - ts);
+                            L += ml[u].y * w;
+#pragma unroll
+                            for (int k = 0; k < 8; k++) {
+                                sum[2 * k] += v[u][k].x * w;
+                                sum[2 * k + 1] += v[u][k].y * w;
+                            }
+                        }
+                }
+                if (into) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) slot_put(into + (8 * d + k) * AT_THREADS + tid, sum[2 * k], sum[2 * k + 1]);
+                } else {
+                    result(d, sum, L);
+                }
             }
-            if (into) keep(into, sum, M, L);
-            else result(sum, L);
+            if (into) slot_put(into + 8 * DT * AT_THREADS + tid, M, L);   // (behind every read of the parts')
         });
     }
 }
@@ -1216,7 +1245,7 @@ static void attn_launch_d(qq_ctx *ctx, const KvBatch &b, const KvAttn &a)
     uint32_t *work = ctx->kv_work;
     // Many rows a sequence: more than two narrow tiles' columns.
     const bool wide = b.row_start && (int64_t)b.n_rows * a.group > (int64_t)2 * AT_COLS * b.n_seqs;
-    const int parts = wide ? wide_parts(ctx) : attn_parts(ctx, D);
+    const int parts = wide ? wide_parts(ctx) : attn_parts(ctx);
     prof_begin(ctx, K_KV_ATTN);
     if (wide && b.s.page_size >= (E::U == 4 ? 32 : 64))
         QQ_LAUNCH(ctx, (kv_attn_wide_kernel<E, D, true>), dim3(parts), dim3(AT_THREADS), shm, b, a, work);
