@@ -64,6 +64,7 @@ constexpr int AW_COLS = 128;
 constexpr int AW_LEAD = 2;
 constexpr int AW_GROUP = 8;
 constexpr int AW_PER_CU = 2;
+constexpr int AW_TILES = 32;     // tiles a call has at least
 static int wide_parts(const qq_ctx *ctx) { return std::min(ctx->num_cus * AW_PER_CU, AT_MAX_PARTS - 1); }
 
 // The workspace, one a context: counters of arrived parts, zero between
@@ -1243,8 +1244,20 @@ static void attn_launch_d(qq_ctx *ctx, const KvBatch &b, const KvAttn &a)
 {
     const size_t shm = at_plan_bytes(b);
     uint32_t *work = ctx->kv_work;
-    // Many rows a sequence: more than two narrow tiles' columns.
-    const bool wide = b.row_start && (int64_t)b.n_rows * a.group > (int64_t)2 * AT_COLS * b.n_seqs;
+    // The form by what the host knows, columns (lengths are on the device): a
+    // quarter of a wide tile or more a sequence, as sequences with few leave it
+    // idle, and AW_TILES tiles or more in all, as fewer are cut into many parts
+    // whose joins cost more than reading keys again for every 16 columns.
+    // Narrow and wide form, us (bf16, 4 heads of 128; fp16, 8 heads of 64):
+    //   64 sequences of 1024, 16 columns each          -          29 and 37
+    //   64 of 1024, 32 columns                     61 and 51      52 and 37
+    //   1 of 2048, 16 tiles / 32 tiles       30 and 63 / 49 and 63    17 and 32 / 28 and 35
+    //   1 of 8192, 16 tiles / 32 tiles       63 and 70 / 137 and 83   35 and 39 / 69 and 45
+    //   1 of 32768, 8 tiles / 32 tiles      108 and 85 / 478 and 173  59 and 47 / 234 and 87
+    //   4 of 8192, 32 tiles                       154 and 84      82 and 48
+    const int64_t columns = (int64_t)b.n_rows * a.group;
+    const bool wide = b.row_start && columns >= (int64_t)AW_COLS / 4 * b.n_seqs &&
+                      columns * b.s.n_kv_heads >= (int64_t)AW_TILES * AW_COLS;
     const int parts = wide ? wide_parts(ctx) : attn_parts(ctx);
     prof_begin(ctx, K_KV_ATTN);
     if (wide && b.s.page_size >= (E::U == 4 ? 32 : 64))

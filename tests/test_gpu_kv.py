@@ -33,6 +33,7 @@ class Batch:
     """Sequences with random keys and values in a pool of scattered pages, and their device copies.
 
     news: new rows per sequence (None: one row each, without row_start)."""
+    PAD = 0     # rows of no sequence behind the others
 
     def __init__(self, lens, news, nq, nkv, dim, typ, ps, seed=0, window=0, sinks=0, fill=np.nan, layers=1, layer=0,
                  spare=3, width=None, qscale=2.0):
@@ -64,8 +65,10 @@ class Batch:
         self.q = (rng.standard_normal((self.n, nq, dim)) * qscale).astype(np.float32)
         self.d_pool, self.d_table = _up(self.pool.raw), _up(self.table)
         self.d_lens, self.d_starts = _up(np.array(lens, np.int32)), _up(self.starts)
-        self.d_q = _up(self.q)
-        self.d_out = torch.full((self.n + 2, nq, dim), 77.0, device="cuda")   # two rows of nobody
+        self.rows = self.n + (self.PAD if news is not None else 0)
+        self.d_q = torch.zeros((self.rows, nq, dim), device="cuda")[:self.n]
+        self.d_q.copy_(_up(self.q))
+        self.d_out = torch.full((self.rows + 2, nq, dim), 77.0, device="cuda")   # two rows of nobody
         self.no_starts = news is None
         torch.cuda.synchronize()
 
@@ -76,7 +79,7 @@ class Batch:
     def batch(self, **over):
         f = dict(n_seqs=len(self.lens), table_ptr=self.d_table.data_ptr(), table_stride=self.width,
                  len_ptr=self.d_lens.data_ptr(), row_start_ptr=None if self.no_starts else self.d_starts.data_ptr(),
-                 n_rows=self.n)
+                 n_rows=self.rows)
         f.update(over)
         return qq_hip.KvBatch(**f)
 
@@ -598,7 +601,7 @@ def test_graphs_follow_lengths_and_tables():
     c = Batch([600, 31, 300], [200, 31, 60], nq, nkv, dim, F16, ps, fill=0.25)
     c.d_pool = b.d_pool
     table = b.table.copy()
-    dk, dv = (torch.randn((c.n, nkv, dim), device="cuda") for _ in range(2))
+    dk, dv = (torch.randn((c.rows, nkv, dim), device="cuda") for _ in range(2))
     kv = b.kv(ctx)
     out = torch.zeros((3, nq, dim), device="cuda")
     torch.cuda.synchronize()
@@ -792,6 +795,68 @@ def test_scores_of_minus_infinity():
                 continue
             ref, bound = attention(b.q[r:r + 1], b.k[0][at], b.v[0][at], np.array([len(at) - 1]), 0.125, 0, 0)
             _check(got[r:r + 1], ref, bound, (news, r))
+
+
+# ---------------------------------------------------------------- the form of large calls
+
+@pytest.fixture
+def large(monkeypatch):
+    """Rows of no sequence fill the calls up to the size that takes the form for many rows."""
+    monkeypatch.setattr(Batch, "PAD", 4096)
+
+
+@pytest.mark.parametrize("typ", sorted(NAMES))
+@pytest.mark.parametrize("heads", HEADS, ids=str)
+def test_large_rows(large, heads, typ):
+    test_rows(heads, typ)
+    test_rows(heads[:2] + (160 - heads[2],), typ)      # another head size, the other page form
+    _run([5, 257, 512, 1000], [5, 1, 12, 200], heads, typ, 128)
+
+
+@pytest.mark.parametrize("typ", sorted(NAMES))
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (5, 3), (64, 4), (100, 40), (250, 1), (31, 700)])
+def test_large_rows_window(large, window, sinks, typ):
+    test_rows_window(window, sinks, typ)
+    _run([257, 30, 700], [257, 30, 200], (4, 1, 128), typ, 64, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("typ", sorted(NAMES))
+def test_large_rows_long(large, typ):
+    test_rows_long((4, 1, 96), 16, typ)
+    test_rows_long((2, 2, 32), 256, typ)
+    test_joined_in_groups([2, 1], (16, 1, 128), typ)
+    test_joined_in_groups([40, 1], (11, 1, 96), typ)
+    test_few_rows_each(typ)
+
+
+@pytest.mark.parametrize("case", [test_rows_ahead_of_position_zero, test_values_that_are_not_finite,
+                                  test_scores_of_minus_infinity, test_graphs_follow_lengths_and_tables,
+                                  lambda: test_pages_that_are_none(True)],
+                         ids=["ahead_of_zero", "not_finite", "minus_infinity", "graphs", "no_pages"])
+def test_large_edges(large, case):
+    case()
+
+
+def test_large_calls_in_turn(monkeypatch):
+    """Both forms, split in many parts, by turns over one workspace."""
+    ctx, forms = gpu_context(), []
+    for i, (lens, news, heads, typ, ps) in enumerate((
+            ([2000], [300], (4, 1, 64), F16, 64), ([9000], None, (4, 1, 64), F16, 64), ([5000], [40], (8, 1, 128), F32, 64),
+            ([9000, 30], None, (8, 2, 128), BF16, 32), ([9000, 100, 7], [3, 1, 2], (4, 1, 32), F16, 16),
+            ([1500], [500], (2, 2, 96), BF16, 16))):
+        monkeypatch.setattr(Batch, "PAD", 4096 if i % 2 == 0 else 0)
+        forms.append(Batch(lens, news, *heads, typ, ps, fill=0.5, seed=i))
+    kvs = [b.kv(ctx) for b in forms]
+    refs = [b.ref(0.1) for b in forms]
+    try:
+        for i in (0, 1, 0, 2, 3, 0, 4, 5, 2, 4, 1, 0, 5, 3, 2):
+            forms[i].d_out.fill_(77.0)
+            _torch().cuda.synchronize()
+            _check(forms[i].attn(ctx, kvs[i], 0.1), *refs[i], i)
+            assert (forms[i].d_out[forms[i].n:] == 77.0).all()
+    finally:
+        for kv in kvs:
+            kv.release()
 
 
 # ---------------------------------------------------------------- together
