@@ -7,6 +7,9 @@
 // lanes idle) and the sum of squares is a shuffle tree over h lanes.  The
 // angle belongs to (row, i), not to the head: a workgroup forms its row's
 // binary64 sines and cosines once, and its waves go through the row's heads.
+// Measured: 64 rows of 32 + 4 heads of 128 5.2 us, a launch and three loads
+// one behind the other; 1470 rows of 32 + 8 heads of 64 13.1 us, 2.5 TB/s,
+// waves waiting two thirds of the time and binary64 half of the rest.
 #include "kv_device.h"
 
 // binary64 expressions of the reference stay separate multiplies and adds
@@ -153,7 +156,7 @@ int launch_kv_store(qq_ctx *ctx, const KvBatch &b, const KvStore &st)
 {
     const int half = b.s.head_dim / 2, hpw = half <= 32 ? WAVE / half : 1;
     const int waves = (st.n_heads + b.s.n_kv_heads + hpw - 1) / hpw;
-    // one pass of a workgroup's waves over the row's heads while rows are few
+    // one pass of a workgroup's waves over the row's heads while rows are few (64 rows 5.2 us, a workgroup a row 10; 1470 rows the same)
     const int gy = std::max(1, std::min((waves + 3) / 4, 1024 / b.n_rows));
     const dim3 grid(b.n_rows, gy);
     prof_begin(ctx, K_KV_STORE);
@@ -169,7 +172,7 @@ int launch_kv_store(qq_ctx *ctx, const KvBatch &b, const KvStore &st)
 
 // Grid (pair, layer, piece): a page of one layer is one run of page_bytes (a
 // multiple of 512), copied in pieces of 16 KiB, four 16-byte loads of a lane in
-// flight.
+// flight: 5.0 TB/s, read and written, for 100 MB, the rate of a large copy.
 constexpr int KV_PIECE = 16384;
 __global__ __launch_bounds__(256) void kv_copy_kernel(char *pool, size_t page_bytes, int n_pages,
                                                       const int32_t *__restrict__ pairs)
